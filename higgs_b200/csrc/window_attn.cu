@@ -1,0 +1,425 @@
+// window_attn.cu -- paged attention through a sliding window with sinks: the query at position p
+// sees key j when j <= p and (j > p - window or j < sinks).  The mask beside those of
+// crates/higgs-models/src/utils.rs:64-125; q, K / V pages and rounding points as in
+// higgs_paged_attention (utils.rs:45-60).
+//
+// Pages wholly behind the window and past the sinks are neither looked up nor read, so a host may
+// free them.  Rows whose position is negative (a query batch longer than its sequence) see nothing
+// and give zeros.
+//
+// Decode kernel (few query rows per kv head).  A CTA takes a split of the visible pages of one
+// (sequence, kv head, tile of query rows = tokens x the G heads of the kv head), its 4 warps
+// alternate over the pages.  The page's 16 keys are the MMA's 16 rows and up to 8 query rows its
+// 8 columns, so G = 4 heads waste half of the tile and not three quarters of it:
+//   S^T = K Q^T     A = K, 16 keys x 16 of d,     B = Q^T
+//   O^T += V^T P^T  A = V^T, 16 of d x 16 keys,   B = P^T
+// Both A operands come straight from global memory, 16 bytes per lane and load, with no shared
+// memory between: the sum over d may run in any order, so a lane's 16 bytes of a K row serve two
+// MMA steps (Q is laid out the same way); and the rows of O^T may be any d, so a lane loads 16
+// bytes of each of its 4 keys of V and pairs the keys with PRMT.  P^T goes from the accumulator's
+// layout to B's by an 8x8 transpose in registers (movmatrix), as bf16 hi + lo halves.  The running
+// maximum moves only when a score exceeds it by 2^kSlack.
+// Bound: HBM, 4 * D bytes per visible key and kv head.
+#include <algorithm>
+
+#include "common.cuh"
+#include "kernels.cuh"
+
+namespace higgs {
+namespace {
+
+constexpr int kWinThreads = 128;
+constexpr int kWinWarps = kWinThreads / 32;
+constexpr int kWinCounterBytes = 16384;
+constexpr int kMaxSplits = 64;
+constexpr int kTargetCtas = 4 * 148;
+static_assert(kTargetCtas / 2 <= kWinCounterBytes / 4, "launches of two splits or more count in the workspace");
+constexpr float kSlack = 8.0f;  // log2
+
+struct WinArgs {
+  const uint16_t* q;
+  const uint16_t* kc;
+  const uint16_t* vc;
+  int64_t page_stride, head_stride;
+  const int32_t* bt;
+  int max_blocks;
+  const int32_t* seq_lens;
+  int Lq, Hq, Hkv, window, sinks;
+  float scale_log2;
+  uint16_t* out;
+  int splits, tiles;
+  int* counters;  // [B * Hkv * tiles] splits done: zero before the launch, zero after it
+  float* part;    // [pairs][splits][rows of a tile][D + 2]: O, then m and l
+};
+
+// The visible pages of a tile of queries at positions p_lo .. p_hi: the sinks' pages, then the
+// window's.  Page i of them is page(i) of the sequence.
+struct Visible {
+  int lo, sink_pages, n;  // lo: first key of the window of p_lo
+  __device__ Visible(int p_lo, int p_hi, int window, int sinks) {
+    lo = max(0, p_lo - window + 1);
+    const int sink_keys = min(sinks, p_hi + 1);
+    sink_pages = min((sink_keys + 15) >> 4, lo >> 4);
+    n = p_hi < 0 ? 0 : sink_pages + (p_hi >> 4) - (lo >> 4) + 1;
+  }
+  __device__ int page(int i) const { return i < sink_pages ? i : i - sink_pages + (lo >> 4); }
+};
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t part4(const uint4& v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+
+__device__ __forceinline__ uint4 ldg16_if(const uint16_t* p, bool ok) {
+  return ok ? ldg_stream_u4(p) : make_uint4(0, 0, 0, 0);
+}
+
+// Row r of the tile as (query token, query head) of the call.
+struct Row {
+  int t, head;
+  __device__ Row(const WinArgs& a, int h, int r) {
+    const int G = a.Hq / a.Hkv;
+    t = r / G;
+    head = h * G + r % G;
+  }
+};
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
+  constexpr int RT = 8 * NT;     // query rows of a tile
+  constexpr int KC = D / 32;     // 16-byte chunks of a K row per lane
+  constexpr int VC = D / 64;     // 16-byte chunks of a V row per lane
+  constexpr int MT = D / 16;     // 16-row tiles of O^T
+  constexpr int QS = D + 8;      // padded row of Q in shared memory
+  __shared__ __align__(16) uint16_t qs[RT * QS];
+  __shared__ float sm_m[kWinWarps][RT], sm_l[kWinWarps][RT];
+  extern __shared__ __align__(16) float sm_o[];  // [warps][RT][D]
+  __shared__ int is_last;
+  const int split = blockIdx.x, h = blockIdx.y / a.tiles, tile = blockIdx.y % a.tiles, b = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int R = (a.Hq / a.Hkv) * a.Lq, r0 = tile * RT, rows = min(RT, R - r0);
+
+  pdl_wait();
+  pdl_launch();
+  const int first = a.seq_lens[b] - a.Lq;  // position of query token 0
+  // (a length beyond the block table would be an error of the caller: no key past it is read)
+  const int p_hi = min(first + Row(a, h, r0 + rows - 1).t, a.max_blocks * 16 - 1);
+  const int p_lo = max(0, first + Row(a, h, r0).t);
+  const Visible vis(p_lo, p_hi, a.window, a.sinks);
+  const int per = (vis.n + a.splits - 1) / a.splits;
+  const int u0 = split * per, u1 = min(vis.n, u0 + per);
+
+  // Q tile, rows past the last one zero
+  for (int i = threadIdx.x; i < RT * (D / 8); i += kWinThreads) {
+    const int r = i / (D / 8), c = i % (D / 8);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (r < rows) {
+      const Row q(a, h, r0 + r);
+      v = *reinterpret_cast<const uint4*>(a.q + (((size_t)b * a.Lq + q.t) * a.Hq + q.head) * D + c * 8);
+    }
+    *reinterpret_cast<uint4*>(qs + r * QS + c * 8) = v;
+  }
+  __syncthreads();
+
+  int pos[NT][2];  // positions of this lane's columns 8 nt + 2 t + {0, 1}
+  float m[NT][2], l[NT][2], o[NT][MT][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = 8 * nt + 2 * t + e;
+      pos[nt][e] = r < rows ? first + Row(a, h, r0 + r).t : -1;
+      m[nt][e] = -INFINITY;
+      l[nt][e] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[nt][j][c] = 0.f;
+  }
+
+  const int32_t* bt = a.bt + (size_t)b * a.max_blocks;
+  const size_t head_off = (size_t)h * a.head_stride;
+  for (int u = u0 + warp; u < u1; u += kWinWarps) {
+    const int pg = vis.page(u);
+    const size_t off = (size_t)bt[pg] * a.page_stride + head_off;
+    const uint16_t* kp = a.kc + off;
+    const uint16_t* vp = a.vc + off;
+    // keys of this page that some query of the tile sees: a hidden key is not loaded, so what its
+    // slot holds does not matter
+    const int j0 = pg * 16;
+    auto seen = [&](int k) { return j0 + k <= p_hi && (j0 + k >= vis.lo || j0 + k < a.sinks); };
+    // every key visible to every query row?
+    const bool inner = j0 + 15 <= p_lo && (j0 > p_hi - a.window || j0 + 15 < a.sinks);
+    uint4 kf[2][KC], vf[4][VC];
+#pragma unroll
+    for (int i = 0; i < KC; ++i) {
+      kf[0][i] = ldg16_if(kp + g * D + (4 * i + t) * 8, inner || seen(g));
+      kf[1][i] = ldg16_if(kp + (g + 8) * D + (4 * i + t) * 8, inner || seen(g + 8));
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int k = 2 * t + (r & 1) + 8 * (r >> 1);
+#pragma unroll
+      for (int c = 0; c < VC; ++c) vf[r][c] = ldg16_if(vp + k * D + 64 * c + g * 8, inner || seen(k));
+    }
+    uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float s[4] = {0.f, 0.f, 0.f, 0.f};  // (key g, column 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1)
+#pragma unroll
+      for (int i = 0; i < KC; ++i) {
+        const uint4 qv = *reinterpret_cast<const uint4*>(qs + (8 * nt + g) * QS + (4 * i + t) * 8);
+        mma_bf16_16816(s, kf[0][i].x, kf[1][i].x, kf[0][i].y, kf[1][i].y, qv.x, qv.y);
+        mma_bf16_16816(s, kf[0][i].z, kf[1][i].z, kf[0][i].w, kf[1][i].w, qv.z, qv.w);
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[c] *= a.scale_log2;
+      if (!inner) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int j = j0 + g + 8 * (c >> 1), p = pos[nt][c & 1];
+          if (!(j <= p && (j > p - a.window || j < a.sinks))) s[c] = -INFINITY;
+        }
+      }
+      const float mx0 = fmaxf(s[0], s[2]), mx1 = fmaxf(s[1], s[3]);
+      if (__any_sync(0xffffffffu, mx0 > m[nt][0] + kSlack || mx1 > m[nt][1] + kSlack)) {
+        float mx[2] = {mx0, mx1}, alpha[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int x = 4; x <= 16; x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
+          const float mn = fmaxf(m[nt][e], mx[e]);
+          alpha[e] = mn == -INFINITY ? 1.f : exp2f(m[nt][e] - mn);
+          m[nt][e] = mn;
+          l[nt][e] *= alpha[e];
+        }
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+          o[nt][j][0] *= alpha[0];
+          o[nt][j][1] *= alpha[1];
+          o[nt][j][2] *= alpha[0];
+          o[nt][j][3] *= alpha[1];
+        }
+      }
+      const float b0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], b1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+      s[0] = exp2f(s[0] - b0);
+      s[1] = exp2f(s[1] - b1);
+      s[2] = exp2f(s[2] - b0);
+      s[3] = exp2f(s[3] - b1);
+      l[nt][0] += s[0] + s[2];
+      l[nt][1] += s[1] + s[3];
+      uint32_t hi, lo;
+      split_bf2(s[0], s[1], hi, lo);
+      ph[nt][0] = transpose8x8(hi);
+      pl[nt][0] = transpose8x8(lo);
+      split_bf2(s[2], s[3], hi, lo);
+      ph[nt][1] = transpose8x8(hi);
+      pl[nt][1] = transpose8x8(lo);
+    }
+    // O^T tile j: rows g and g + 8 are d = 8 g + j and, 128 wide, 64 + 8 g + j; 64 wide, 8 g + j + 4
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      const int c1 = VC - 1, e1 = VC == 2 ? j : j + 4;
+      const uint32_t sel0 = (j & 1) ? 0x7632u : 0x5410u, sel1 = (e1 & 1) ? 0x7632u : 0x5410u;
+      const uint32_t a0 = prmt(part4(vf[0][0], j >> 1), part4(vf[1][0], j >> 1), sel0);
+      const uint32_t a1 = prmt(part4(vf[0][c1], e1 >> 1), part4(vf[1][c1], e1 >> 1), sel1);
+      const uint32_t a2 = prmt(part4(vf[2][0], j >> 1), part4(vf[3][0], j >> 1), sel0);
+      const uint32_t a3 = prmt(part4(vf[2][c1], e1 >> 1), part4(vf[3][c1], e1 >> 1), sel1);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        mma_bf16_16816(o[nt][j], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
+        mma_bf16_16816(o[nt][j], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
+      }
+    }
+  }
+
+  // ---- the warps' shares of the split, in shared memory ----
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float lv = l[nt][e];
+#pragma unroll
+      for (int x = 4; x <= 16; x <<= 1) lv += __shfl_xor_sync(0xffffffffu, lv, x);
+      const int r = 8 * nt + 2 * t + e;
+      if (g == 0) {
+        sm_m[warp][r] = m[nt][e];
+        sm_l[warp][r] = lv;
+      }
+      float* dst = sm_o + (warp * RT + r) * D;
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        dst[8 * g + j] = o[nt][j][e];
+        dst[D == 128 ? 64 + 8 * g + j : 8 * g + j + 4] = o[nt][j][2 + e];
+      }
+    }
+  __syncthreads();
+  const int pair = (b * a.Hkv + h) * a.tiles + tile;
+  float* part = a.part + ((size_t)pair * a.splits + split) * RT * (D + 2);
+  auto store = [&](int r, int d, float v) {
+    const Row q(a, h, r0 + r);
+    a.out[(((size_t)b * a.Lq + q.t) * a.Hq + q.head) * D + d] = f2bf(first + q.t >= 0 ? v : 0.f);
+  };
+  for (int i = threadIdx.x; i < rows * D; i += kWinThreads) {
+    const int r = i / D, d = i % D;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWinWarps; ++w) M = fmaxf(M, sm_m[w][r]);
+    float L = 0.f, O = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWinWarps; ++w) {
+      const float f = sm_m[w][r] == -INFINITY ? 0.f : exp2f(sm_m[w][r] - M);
+      L = fmaf(f, sm_l[w][r], L);
+      O = fmaf(f, sm_o[(w * RT + r) * D + d], O);
+    }
+    if (a.splits == 1) {
+      store(r, d, L > 0.f ? O / L : 0.f);
+    } else {
+      part[r * (D + 2) + d] = O;
+      if (d == 0) {
+        part[r * (D + 2) + D] = M;
+        part[r * (D + 2) + D + 1] = L;
+      }
+    }
+  }
+  if (a.splits == 1) return;
+
+  // ---- the last split to finish joins them, in the order of the splits ----
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) is_last = atomicAdd(a.counters + pair, 1) == a.splits - 1;
+  __syncthreads();
+  if (!is_last) return;
+  __threadfence();
+  const float* parts = a.part + (size_t)pair * a.splits * RT * (D + 2);
+  for (int i = threadIdx.x; i < rows * D; i += kWinThreads) {
+    const int r = i / D, d = i % D;
+    const float* p = parts + r * (D + 2);
+    float M = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, __ldcg(p + (size_t)s * RT * (D + 2) + D));
+    float L = 0.f, O = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+      const float* q = p + (size_t)s * RT * (D + 2);
+      const float ms = __ldcg(q + D);
+      const float f = ms == -INFINITY ? 0.f : exp2f(ms - M);
+      L = fmaf(f, __ldcg(q + D + 1), L);
+      O = fmaf(f, __ldcg(q + d), O);
+    }
+    store(r, d, L > 0.f ? O / L : 0.f);
+  }
+  if (threadIdx.x == 0) a.counters[pair] = 0;
+}
+
+struct WinPlan {
+  int nt, tiles, splits;
+};
+
+// Row tiles of 8, 16 or 32 query rows; splits of the longest visible range so that the CTAs fill
+// the GPU, four pages (one per warp) at least.
+WinPlan plan_window(int B, int Lq, int Hq, int Hkv, int max_seq_len, int window, int sinks) {
+  WinPlan p;
+  const int R = (Hq / Hkv) * Lq;
+  p.nt = R <= 8 ? 1 : R <= 16 ? 2 : 4;
+  p.tiles = (R + 8 * p.nt - 1) / (8 * p.nt);
+  const int64_t keys = std::min<int64_t>(max_seq_len, (int64_t)window + Lq + sinks);
+  const int pages = (int)std::min<int64_t>((max_seq_len + 15) / 16, (keys + 15) / 16 + 2);
+  const int64_t pairs = (int64_t)B * Hkv * p.tiles;
+  const int64_t want = std::max<int64_t>(1, kTargetCtas / pairs);
+  p.splits = (int)std::min<int64_t>(std::min<int64_t>(want, kMaxSplits), std::max(1, (pages + 3) / 4));
+  return p;
+}
+
+size_t window_ws_bytes(const WinPlan& p, int B, int Hkv, int D) {
+  if (p.splits == 1) return kWinCounterBytes;
+  return kWinCounterBytes + (size_t)B * Hkv * p.tiles * p.splits * 8 * p.nt * (D + 2) * sizeof(float);
+}
+
+bool window_shape_ok(int B, int Lq, int Hq, int Hkv, int D, int max_seq_len, int window, int sinks) {
+  return B > 0 && Lq > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && (D == 64 || D == 128) && max_seq_len > 0 &&
+         max_seq_len <= (1 << 30) && window > 0 && sinks >= 0 && (int64_t)Lq * Hq <= (1 << 30) && Hkv <= 65535 &&
+         B <= 65535;
+}
+
+template <int D, int NT>
+cudaError_t launch_window(const WinArgs& a, int B, cudaStream_t st) {
+  auto k = window_decode_kernel<D, NT>;
+  const size_t smem = (size_t)kWinWarps * 8 * NT * D * sizeof(float);
+  static PerDeviceOnce attr;
+  const cudaError_t e =
+      attr.run([&] { return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); });
+  if (e != cudaSuccess) return e;
+  return launch_pdl(k, dim3(a.splits, a.Hkv * a.tiles, B), dim3(kWinThreads), smem, st, a);
+}
+
+}  // namespace
+}  // namespace higgs
+
+using namespace higgs;
+
+extern "C" size_t higgs_window_attention_workspace_size(int B, int Lq, int Hq, int Hkv, int D, int max_seq_len,
+                                                        int window, int sinks) {
+  if (!window_shape_ok(B, Lq, Hq, Hkv, D, max_seq_len, window, sinks)) return 0;
+  return window_ws_bytes(plan_window(B, Lq, Hq, Hkv, max_seq_len, window, sinks), B, Hkv, D);
+}
+
+extern "C" int higgs_window_attention(higgs_ctx* ctx, const void* q, int B, int Lq, int Hq, int Hkv, int D,
+                                      const void* k_cache, const void* v_cache, int64_t page_stride,
+                                      int64_t head_stride, const int32_t* block_table, int max_blocks,
+                                      const int32_t* seq_lens, int max_seq_len, int window, int sinks, float scale,
+                                      void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  HG_CHECK_ARG(ctx && q && k_cache && v_cache && block_table && seq_lens && out && workspace,
+               "higgs_window_attention: null argument");
+  HG_CHECK_ARG(D == 64 || D == 128, "higgs_window_attention: D must be 64 or 128");
+  HG_CHECK_ARG(window > 0 && sinks >= 0, "higgs_window_attention: needs window >= 1 and sinks >= 0");
+  HG_CHECK_ARG(window_shape_ok(B, Lq, Hq, Hkv, D, max_seq_len, window, sinks),
+               "higgs_window_attention: bad batch / head shape");
+  HG_CHECK_ARG((int64_t)max_blocks * HIGGS_PAGE_SIZE >= max_seq_len && max_blocks <= (1 << 26),
+               "higgs_window_attention: block table too short (or beyond 2^26 pages)");
+  HG_CHECK_ARG((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)workspace) &
+                15) == 0 &&
+                   page_stride % 8 == 0 && head_stride % 8 == 0,
+               "higgs_window_attention: tensors, workspace and strides must be 16-byte aligned");
+  const WinPlan p = plan_window(B, Lq, Hq, Hkv, max_seq_len, window, sinks);
+  HG_CHECK_ARG((int64_t)Hkv * p.tiles <= 65535, "higgs_window_attention: too many query rows");
+  const size_t need = window_ws_bytes(p, B, Hkv, D);
+  if (workspace_bytes < need)
+    return fail(HIGGS_ERR_WORKSPACE,
+                "higgs_window_attention: workspace too small (need " + std::to_string(need) + " bytes)");
+  HG_DEVICE(ctx);
+  WinArgs a;
+  a.q = (const uint16_t*)q;
+  a.kc = (const uint16_t*)k_cache;
+  a.vc = (const uint16_t*)v_cache;
+  a.page_stride = page_stride;
+  a.head_stride = head_stride;
+  a.bt = block_table;
+  a.max_blocks = max_blocks;
+  a.seq_lens = seq_lens;
+  a.Lq = Lq;
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.window = window;
+  a.sinks = sinks;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = (uint16_t*)out;
+  a.splits = p.splits;
+  a.tiles = p.tiles;
+  a.counters = (int*)workspace;
+  a.part = (float*)((char*)workspace + kWinCounterBytes);
+  cudaStream_t st = (cudaStream_t)stream;
+  cudaError_t e;
+  if (D == 64)
+    e = p.nt == 1 ? launch_window<64, 1>(a, B, st) : p.nt == 2 ? launch_window<64, 2>(a, B, st)
+                                                               : launch_window<64, 4>(a, B, st);
+  else
+    e = p.nt == 1 ? launch_window<128, 1>(a, B, st) : p.nt == 2 ? launch_window<128, 2>(a, B, st)
+                                                                : launch_window<128, 4>(a, B, st);
+  HG_CUDA(e);
+  return HIGGS_OK;
+}

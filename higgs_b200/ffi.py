@@ -44,6 +44,9 @@ SIGNATURES: dict[str, tuple] = {
     "higgs_fused_attention_workspace_size": (SZ, [I, I, I, I, I, I]),
     "higgs_fused_attention": (I, [P, P, I, I, I, I, I, P, P, F, P, P, P, P, P, I64, I64, P, I, P, I, F, P, P, SZ, P]),
     "higgs_paged_attention_noalloc": (I, [P, P, I, I, I, I, I, P, P, I64, I64, P, I, P, I, F, P, P]),
+    "higgs_window_attention_workspace_size": (SZ, [I, I, I, I, I, I, I, I]),
+    "higgs_window_attention": (I, [P, P, I, I, I, I, I, P, P, I64, I64, P, I, P, I, I, I, F, P, P, SZ, P]),
+    "higgs_kv_copy_pages": (I, [P, P, I, P, P, I, P]),
     "higgs_tq4_encode": (I, [P, P, I64, P, P, P, P]),
     "higgs_qknorm_rope_kv_write_tq4": (I, [P, P, I, I, I, P, P, F, P, P, P, P, P, P, P, P, I64, I64, P, P]),
     "higgs_paged_attention_tq4_workspace_size": (SZ, [I, I, I, I, I]),
@@ -55,6 +58,8 @@ SIGNATURES: dict[str, tuple] = {
     "higgs_sample_filtered": (I, [P, P, I, I, F, I, F, F, P, P, P]),
     "higgs_logprobs": (I, [P, P, I, I, F, P, I, P, P, P, P]),
     "higgs_apply_token_mask": (I, [P, P, I, I, P, I, P]),
+    "higgs_beam_select_workspace_size": (SZ, [I, I, I, I]),
+    "higgs_beam_select": (I, [P, P, P, I, I, I, I, P, P, P, P, SZ, P]),
     "higgs_rmsnorm_strided": (I, [P, P, I64, I, I, P, F, P, P]),
     "higgs_moe_plan_size": (SZ, [I, I, I]),
     "higgs_moe_route_topk": (I, [P, P, I, I, I, I, I, P, P, P, SZ, P]),
@@ -110,6 +115,12 @@ class ChainGemv(ctypes.Structure):
     _fields_ = [("x", P), ("norm_w", P), ("K", I), ("N", I), ("swiglu", I), ("nseg", I),
                 ("seg_end", I * 3), ("w", P * 3), ("s", P * 3), ("b", P * 3), ("w2", P), ("s2", P),
                 ("b2", P), ("y", P), ("y_f32", P), ("residual", P)]
+
+
+class KvPool(ctypes.Structure):
+    """higgs_kv_pool (include/higgs_cuda.h)."""
+    _fields_ = [("base", P), ("layers", I), ("num_pages", I64), ("layer_stride", I64),
+                ("page_stride", I64), ("page_bytes", I64)]
 
 
 class ModelConfig(ctypes.Structure):

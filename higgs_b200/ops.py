@@ -7,8 +7,10 @@ Reference call sites are cited per function.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
+import numpy as np
 import torch
 
 from . import ffi
@@ -35,6 +37,12 @@ def _chk(t: torch.Tensor, dtype, name: str):
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+
+
+def _same_device(x: torch.Tensor, **others):
+    for name, t in others.items():
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, not on {x.device}")
 
 
 # ---- a1/a2 ----------------------------------------------------------------
@@ -282,6 +290,74 @@ def fused_attention(qkv, Hq: int, Hkv: int, D: int, q_norm_w, k_norm_w, eps: flo
     return out
 
 
+def window_attention_workspace(B, Lq, Hq, Hkv, D, max_seq_len, window, sinks, device) -> torch.Tensor:
+    n = ffi.load().higgs_window_attention_workspace_size(B, Lq, Hq, Hkv, D, max_seq_len, window, sinks)
+    return torch.zeros(max(n, 16384), dtype=torch.uint8, device=device)
+
+
+def window_attention(q, k_cache, v_cache, block_table, seq_lens, max_seq_len: int, window: int,
+                     sinks: int = 0, scale=None, workspace=None):
+    """Paged attention in which query position p sees key j when j <= p and (j > p - window or
+    j < sinks); see higgs_window_attention.
+
+    q bf16 [B, Lq, Hq, D], contiguous; caches bf16 [num_pages, Hkv, 16, D], of equal strides, each
+    (page, head) block contiguous; block_table int32 [B, max_blocks], whose entries of pages no
+    query sees may hold anything; seq_lens int32 [B], at most max_seq_len.  Returns bf16 [B, Lq, Hq, D]."""
+    _chk(q, torch.bfloat16, "q")
+    _chk(block_table, torch.int32, "block_table")
+    _chk(seq_lens, torch.int32, "seq_lens")
+    if q.dim() != 4 or k_cache.dim() != 4:
+        raise ValueError("q must be [B, Lq, Hq, D] and the caches [num_pages, Hkv, 16, D]")
+    B, Lq, Hq, D = q.shape
+    Hkv = k_cache.shape[1]
+    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if c.dtype != torch.bfloat16:
+            raise TypeError(f"{name} must be torch.bfloat16, got {c.dtype}")
+        if c.shape != k_cache.shape or tuple(c.shape[2:]) != (PAGE, D):
+            raise ValueError(f"{name} must be [num_pages, Hkv, {PAGE}, {D}], got {list(c.shape)}")
+        if c.stride() != k_cache.stride() or c.stride()[2:] != (D, 1):
+            raise ValueError("the caches need equal strides and contiguous (page, head) blocks")
+    if block_table.dim() != 2 or block_table.shape[0] != B or tuple(seq_lens.shape) != (B,):
+        raise ValueError("block_table must be [B, max_blocks] and seq_lens [B]")
+    ctx = _ctx(q)
+    _same_device(q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, seq_lens=seq_lens,
+                 workspace=workspace)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    if workspace is None:
+        workspace = window_attention_workspace(B, Lq, Hq, Hkv, D, int(max_seq_len), int(window), int(sinks),
+                                               q.device)
+    out = torch.empty_like(q)
+    ffi.call("higgs_window_attention", ctx, _p(q), B, Lq, Hq, Hkv, D, _p(k_cache), _p(v_cache),
+             k_cache.stride(0), k_cache.stride(1), _p(block_table), block_table.shape[1], _p(seq_lens),
+             int(max_seq_len), int(window), int(sinks), float(scale), _p(out), _p(workspace),
+             workspace.numel(), _st(q.device))
+    return out
+
+
+def kv_copy_pages(pools, src, dst) -> None:
+    """In every tensor [layers, num_pages, ...] of ``pools`` and every layer of it, page dst[i]
+    becomes page src[i]; see higgs_kv_copy_pages.  The tensors are a cache's K and V (or its codes
+    and scales), each page contiguous; src and dst are host lists of page ids."""
+    pools = list(pools)
+    if not pools:
+        raise ValueError("kv_copy_pages: no pools")
+    src, dst = (np.ascontiguousarray(a, dtype=np.int32).reshape(-1) for a in (src, dst))
+    if src.size != dst.size:
+        raise ValueError(f"kv_copy_pages: {src.size} sources, {dst.size} destinations")
+    arr = (ffi.KvPool * len(pools))()
+    for a, t in zip(arr, pools):
+        if t.dim() < 3 or not t[0, 0].is_contiguous():
+            raise ValueError("a pool must be [layers, num_pages, ...] with contiguous pages")
+        _same_device(pools[0], pool=t)
+        es = t.element_size()
+        a.base, a.layers, a.num_pages = _p(t), t.shape[0], t.shape[1]
+        a.layer_stride, a.page_stride = t.stride(0) * es, t.stride(1) * es
+        a.page_bytes = math.prod(t.shape[2:]) * es
+    ffi.call("higgs_kv_copy_pages", _ctx(pools[0]), arr, len(pools), src.ctypes.data_as(ctypes.c_void_p),
+             dst.ctypes.data_as(ctypes.c_void_p), src.size, _st(pools[0].device))
+
+
 def tq4_encode(x, signs):
     """TurboQuant encode of bf16 [n, 128] -> (codes u8 [n, 64], scales fp16 [n])."""
     n = x.numel() // 128
@@ -367,6 +443,38 @@ def logprobs(logits, temperature: float, tokens, top_n: int = 0):
     ffi.call("higgs_logprobs", _ctx(logits), _p(logits), B, V, float(temperature), _p(tokens),
              int(top_n), _p(lp), _p(ids) if top_n else None, _p(tl) if top_n else None, _st(dev))
     return lp, ids, tl
+
+
+def beam_select_workspace(B: int, beams: int, V: int, n_out: int, device) -> torch.Tensor:
+    n = ffi.load().higgs_beam_select_workspace_size(B, beams, V, n_out)
+    return torch.zeros(max(n, 4096), dtype=torch.uint8, device=device)
+
+
+def beam_select(logits, scores, n_out: int, workspace=None):
+    """Beam search's selection: of every request the n_out largest scores[b, w] +
+    log_softmax(logits[b, w])[v], best first, ties to the lower w * V + v; see higgs_beam_select.
+
+    logits f32 [B * beams, V] or [B, beams, V]; scores f32 [B, beams].  Returns (scores f32, beams
+    int32, tokens int32), each [B, n_out]; (-inf, -1, -1) where candidates run out."""
+    _chk(logits, torch.float32, "logits")
+    _chk(scores, torch.float32, "scores")
+    if scores.dim() != 2:
+        raise ValueError("scores must be [B, beams]")
+    B, W = scores.shape
+    V = logits.shape[-1]
+    if logits.numel() != B * W * V:
+        raise ValueError(f"logits must hold {B} x {W} rows, got {list(logits.shape)}")
+    ctx = _ctx(logits)
+    _same_device(logits, scores=scores, workspace=workspace)
+    if workspace is None:
+        workspace = beam_select_workspace(B, W, V, int(n_out), logits.device)
+    dev = logits.device
+    best = torch.empty(B, max(int(n_out), 0), dtype=torch.float32, device=dev)
+    beams = torch.empty(best.shape, dtype=torch.int32, device=dev)
+    tokens = torch.empty(best.shape, dtype=torch.int32, device=dev)
+    ffi.call("higgs_beam_select", ctx, _p(logits), _p(scores), B, W, V, int(n_out), _p(best), _p(beams),
+             _p(tokens), _p(workspace), workspace.numel(), _st(dev))
+    return best, beams, tokens
 
 
 def apply_token_mask(logits, allowed_bits):
@@ -474,7 +582,6 @@ def tc_mma_rate(n: int, nacc: int = 1, spread: int = 0, iters: int = 4096, commi
     """Tensor-core issue rate of the matrix-form quantized matmul's instruction stream
     (higgs_diag_tc_mma_rate): SM cycles per tcgen05.mma m x n x 16 over all issuing warps,
     median over one CTA per SM.  Synchronising."""
-    import ctypes
     dev = torch.device(device)
     if ctas is None:
         ctas = torch.cuda.get_device_properties(dev).multi_processor_count

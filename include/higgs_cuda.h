@@ -371,6 +371,54 @@ int higgs_paged_attention_noalloc(higgs_ctx* ctx, const void* q, int B, int Lq, 
                                   const int32_t* seq_lens, int max_seq_len, float scale, void* out,
                                   void* stream);
 
+/* Attention through a sliding window with sinks over the paged cache (no reference
+ * counterpart: its masks, crates/higgs-models/src/utils.rs:64-125, are causal and
+ * padding masks).  Arguments as in higgs_paged_attention; query t of sequence b sits
+ * at position p = seq_lens[b] - Lq + t and attends to key j when j <= p and
+ * (j > p - window or j < sinks): the last `window` keys, its own among them, and the
+ * first `sinks` keys of the sequence.  window >= 1, sinks >= 0; a window of at least
+ * max_seq_len is the causal mask.
+ *   Rows with p < 0 (Lq above the sequence's length: a batch padded in front, or an
+ *   empty sequence) see no key and give zeros.
+ *   Pages whose keys no query of the call sees are not read, and neither are their
+ *   block_table entries: a host may free those pages and leave any value there.  The
+ *   slots of hidden keys in other pages may hold anything; K and V of a key that some
+ *   query of the call sees must be finite.
+ *   D = 64 or 128; Hq / Hkv any whole number.  Base pointers and strides must be
+ *   multiples of 16 bytes.  workspace: at least
+ *   higgs_window_attention_workspace_size() bytes (0 for a shape that is refused),
+ *   zero-filled before its first use; each call leaves its counters (the first 16384
+ *   bytes) zero, so calls of any shapes that follow one another on a stream can share
+ *   a workspace of the largest size; calls that may run at the same time cannot. */
+size_t higgs_window_attention_workspace_size(int B, int Lq, int Hq, int Hkv, int D,
+                                             int max_seq_len, int window, int sinks);
+int higgs_window_attention(higgs_ctx* ctx, const void* q, int B, int Lq, int Hq, int Hkv, int D,
+                           const void* k_cache, const void* v_cache, int64_t page_stride,
+                           int64_t head_stride, const int32_t* block_table, int max_blocks,
+                           const int32_t* seq_lens, int max_seq_len, int window, int sinks,
+                           float scale, void* out, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
+/* Copies of whole pages inside a cache (the reference clones whole caches,
+ * crates/higgs-engine/src/prompt_cache.rs:186-224): in every pool and every layer of
+ * it, page dst[i] becomes page src[i], i < n.  A pool is one tensor of the cache -- K
+ * or V, or a TurboQuant cache's codes and scales -- with page p of layer l at
+ * base + l * layer_stride + p * page_stride, page_bytes long (bytes; base, strides and
+ * page_bytes multiples of 16; num_pages bounds the ids); 1 to 8 pools that do not
+ * overlap.
+ *   src and dst are HOST lists (page ids come from the host's block pool), read before
+ *   the call returns; a captured graph keeps the lists it was captured with.  A source
+ *   may feed several destinations; a page that is a destination twice, or a source and
+ *   a destination, is refused.  n may be 0. */
+typedef struct {
+  void* base;
+  int layers;
+  int64_t num_pages;
+  int64_t layer_stride, page_stride, page_bytes;
+} higgs_kv_pool;
+int higgs_kv_copy_pages(higgs_ctx* ctx, const higgs_kv_pool* pools, int n_pools,
+                        const int32_t* src, const int32_t* dst, int n, void* stream);
+
 /* ---- a14: TurboQuant-style 4-bit KV (no reference counterpart; the
  * KeyValueCache trait only reserves is_quantized/group_size/bits hooks,
  * crates/higgs-models/src/cache.rs:4-18) ------------------------------------ */
@@ -469,6 +517,24 @@ int higgs_logprobs(higgs_ctx* ctx, const float* logits, int B, int V, float temp
  * FSM each step, as in the reference. */
 int higgs_apply_token_mask(higgs_ctx* ctx, float* logits, int B, int V, const uint32_t* allowed,
                            int words_per_row, void* stream);
+
+/* Beam search's selection (no reference counterpart): for every request b the n_out
+ * best continuations by
+ *   key(w, v) = scores[b, w] + logits[b, w, v] - log sum_u exp(logits[b, w, u]),
+ * best first, ties to the lower w * V + v.  logits f32 [B * beams, V]; scores f32
+ * [B, beams], the beams' log-probabilities so far; out_scores f32 (keys computed in 64
+ * bits and rounded once), out_beams int32 (w) and out_tokens int32 (v), [B, n_out].
+ *   A NaN logit counts as -inf: no mass, never chosen.  A beam whose score is not
+ *   finite, or whose row has no finite maximum, gives no candidates and its row is not
+ *   read (so the first step of a search sets all scores but one to -inf).  Where fewer
+ *   than n_out candidates have a key above -inf the rest are (-inf, -1, -1).
+ *   B <= 1024, beams <= 32, V <= 163840, n_out <= 32.  workspace: at least
+ *   higgs_beam_select_workspace_size() bytes (0 for a shape that is refused), 16-byte
+ *   aligned, its first 4096 bytes zero before the first call and left zero by each. */
+size_t higgs_beam_select_workspace_size(int B, int beams, int V, int n_out);
+int higgs_beam_select(higgs_ctx* ctx, const float* logits, const float* scores, int B, int beams,
+                      int V, int n_out, float* out_scores, int32_t* out_beams,
+                      int32_t* out_tokens, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- a9: mixture of experts (qwen3_moe.rs Qwen3MoeMlpBlock) ------------- */
 
