@@ -49,7 +49,8 @@ struct WinArgs {
   uint16_t* out;
   int splits, tiles;
   int* counters;  // [B * Hkv * tiles] splits done: zero before the launch, zero after it
-  float* part;    // [pairs][splits][rows of a tile][D + 2]: O, then m and l
+  float* part;      // [pairs][splits][rows of a tile][D]: sums of the splits
+  float2* part_ml;  // [pairs][splits][rows of a tile]: their maxima and norms
 };
 
 // The visible pages of a tile of queries at positions p_lo .. p_hi: the sinks' pages, then the
@@ -97,8 +98,9 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
   constexpr int MT = D / 16;     // 16-row tiles of O^T
   constexpr int QS = D + 8;      // padded row of Q in shared memory
   __shared__ __align__(16) uint16_t qs[RT * QS];
-  __shared__ float sm_m[kWinWarps][RT], sm_l[kWinWarps][RT];
-  extern __shared__ __align__(16) float sm_o[];  // [warps][RT][D]
+  __shared__ float2 sm_ml[kWinWarps][RT];  // maximum, norm
+  __shared__ float sm_f[kWinWarps][RT];
+  extern __shared__ __align__(16) float sm_o[];  // [warps][RT][D + 4]
   __shared__ int is_last;
   const int split = blockIdx.x, h = blockIdx.y / a.tiles, tile = blockIdx.y % a.tiles, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -114,6 +116,44 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
   const int per = (vis.n + a.splits - 1) / a.splits;
   const int u0 = split * per, u1 = min(vis.n, u0 + per);
 
+  // A page's K and V loads are issued as soon as the registers of the page before are used up --
+  // K's after its scores, V's after its share of O -- so they are in flight during the rest of
+  // that page; page ids are fetched one page further ahead.
+  const int32_t* bt = a.bt + (size_t)b * a.max_blocks;
+  const size_t head_off = (size_t)h * a.head_stride;
+  uint4 kf[2][KC], vf[4][VC];
+  // keys of a page that some query of the tile sees: a hidden key is not loaded, so what its slot
+  // holds does not matter
+  auto seen = [&](int j) { return j <= p_hi && (j >= vis.lo || j < a.sinks); };
+  // every key of the page visible to every query row
+  auto inner = [&](int j0) { return j0 + 15 <= p_lo && (j0 > p_hi - a.window || j0 + 15 < a.sinks); };
+  auto load_k = [&](int j0, int pid) {
+    const uint16_t* kp = a.kc + (size_t)pid * a.page_stride + head_off + g * D + t * 8;
+    const bool in = inner(j0), s0 = in || seen(j0 + g), s1 = in || seen(j0 + g + 8);
+#pragma unroll
+    for (int i = 0; i < KC; ++i) {
+      kf[0][i] = ldg16_if(kp + 32 * i, s0);
+      kf[1][i] = ldg16_if(kp + 8 * D + 32 * i, s1);
+    }
+  };
+  auto load_v = [&](int j0, int pid) {
+    const uint16_t* vp = a.vc + (size_t)pid * a.page_stride + head_off + 2 * t * D + g * 8;
+    const bool in = inner(j0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int k = (r & 1) + 8 * (r >> 1);
+      const bool ok = in || seen(j0 + 2 * t + k);
+#pragma unroll
+      for (int c = 0; c < VC; ++c) vf[r][c] = ldg16_if(vp + k * D + 64 * c, ok);
+    }
+  };
+  int u = u0 + warp;
+  int pid = u < u1 ? bt[vis.page(u)] : 0, pid_next = u + kWinWarps < u1 ? bt[vis.page(u + kWinWarps)] : 0;
+  if (u < u1) {
+    load_k(vis.page(u) * 16, pid);
+    load_v(vis.page(u) * 16, pid);
+  }
+
   // Q tile, rows past the last one zero
   for (int i = threadIdx.x; i < RT * (D / 8); i += kWinThreads) {
     const int r = i / (D / 8), c = i % (D / 8);
@@ -124,8 +164,6 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
     }
     *reinterpret_cast<uint4*>(qs + r * QS + c * 8) = v;
   }
-  __syncthreads();
-
   int pos[NT][2];  // positions of this lane's columns 8 nt + 2 t + {0, 1}
   float m[NT][2], l[NT][2], o[NT][MT][4];
 #pragma unroll
@@ -142,54 +180,42 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) o[nt][j][c] = 0.f;
   }
+  __syncthreads();
 
-  const int32_t* bt = a.bt + (size_t)b * a.max_blocks;
-  const size_t head_off = (size_t)h * a.head_stride;
-  for (int u = u0 + warp; u < u1; u += kWinWarps) {
-    const int pg = vis.page(u);
-    const size_t off = (size_t)bt[pg] * a.page_stride + head_off;
-    const uint16_t* kp = a.kc + off;
-    const uint16_t* vp = a.vc + off;
-    // keys of this page that some query of the tile sees: a hidden key is not loaded, so what its
-    // slot holds does not matter
-    const int j0 = pg * 16;
-    auto seen = [&](int k) { return j0 + k <= p_hi && (j0 + k >= vis.lo || j0 + k < a.sinks); };
-    // every key visible to every query row?
-    const bool inner = j0 + 15 <= p_lo && (j0 > p_hi - a.window || j0 + 15 < a.sinks);
-    uint4 kf[2][KC], vf[4][VC];
-#pragma unroll
-    for (int i = 0; i < KC; ++i) {
-      kf[0][i] = ldg16_if(kp + g * D + (4 * i + t) * 8, inner || seen(g));
-      kf[1][i] = ldg16_if(kp + (g + 8) * D + (4 * i + t) * 8, inner || seen(g + 8));
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int k = 2 * t + (r & 1) + 8 * (r >> 1);
-#pragma unroll
-      for (int c = 0; c < VC; ++c) vf[r][c] = ldg16_if(vp + k * D + 64 * c + g * 8, inner || seen(k));
-    }
-    uint32_t ph[NT][2], pl[NT][2];
+  for (; u < u1; u += kWinWarps) {
+    const int j0 = vis.page(u) * 16;
+    const bool more = u + kWinWarps < u1, in = inner(j0);
+    const int j0_next = more ? vis.page(u + kWinWarps) * 16 : 0;
+    pid = pid_next;
+    if (u + 2 * kWinWarps < u1) pid_next = bt[vis.page(u + 2 * kWinWarps)];
+    float s[NT][4];  // (key g, column 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float s[4] = {0.f, 0.f, 0.f, 0.f};  // (key g, column 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[nt][c] = 0.f;
 #pragma unroll
       for (int i = 0; i < KC; ++i) {
         const uint4 qv = *reinterpret_cast<const uint4*>(qs + (8 * nt + g) * QS + (4 * i + t) * 8);
-        mma_bf16_16816(s, kf[0][i].x, kf[1][i].x, kf[0][i].y, kf[1][i].y, qv.x, qv.y);
-        mma_bf16_16816(s, kf[0][i].z, kf[1][i].z, kf[0][i].w, kf[1][i].w, qv.z, qv.w);
+        mma_bf16_16816(s[nt], kf[0][i].x, kf[1][i].x, kf[0][i].y, kf[1][i].y, qv.x, qv.y);
+        mma_bf16_16816(s[nt], kf[0][i].z, kf[1][i].z, kf[0][i].w, kf[1][i].w, qv.z, qv.w);
       }
+    }
+    if (more) load_k(j0_next, pid);
+    uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) s[c] *= a.scale_log2;
-      if (!inner) {
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[nt][c] *= a.scale_log2;
+      if (!in) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const int j = j0 + g + 8 * (c >> 1), p = pos[nt][c & 1];
-          if (!(j <= p && (j > p - a.window || j < a.sinks))) s[c] = -INFINITY;
+          if (!(j <= p && (j > p - a.window || j < a.sinks))) s[nt][c] = -INFINITY;
         }
       }
-      const float mx0 = fmaxf(s[0], s[2]), mx1 = fmaxf(s[1], s[3]);
-      if (__any_sync(0xffffffffu, mx0 > m[nt][0] + kSlack || mx1 > m[nt][1] + kSlack)) {
-        float mx[2] = {mx0, mx1}, alpha[2];
+      float mx[2] = {fmaxf(s[nt][0], s[nt][2]), fmaxf(s[nt][1], s[nt][3])};
+      if (__any_sync(0xffffffffu, mx[0] > m[nt][0] + kSlack || mx[1] > m[nt][1] + kSlack)) {
+        float alpha[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
@@ -208,17 +234,17 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
         }
       }
       const float b0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], b1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
-      s[0] = exp2f(s[0] - b0);
-      s[1] = exp2f(s[1] - b1);
-      s[2] = exp2f(s[2] - b0);
-      s[3] = exp2f(s[3] - b1);
-      l[nt][0] += s[0] + s[2];
-      l[nt][1] += s[1] + s[3];
+      s[nt][0] = exp2f(s[nt][0] - b0);
+      s[nt][1] = exp2f(s[nt][1] - b1);
+      s[nt][2] = exp2f(s[nt][2] - b0);
+      s[nt][3] = exp2f(s[nt][3] - b1);
+      l[nt][0] += s[nt][0] + s[nt][2];
+      l[nt][1] += s[nt][1] + s[nt][3];
       uint32_t hi, lo;
-      split_bf2(s[0], s[1], hi, lo);
+      split_bf2(s[nt][0], s[nt][1], hi, lo);
       ph[nt][0] = transpose8x8(hi);
       pl[nt][0] = transpose8x8(lo);
-      split_bf2(s[2], s[3], hi, lo);
+      split_bf2(s[nt][2], s[nt][3], hi, lo);
       ph[nt][1] = transpose8x8(hi);
       pl[nt][1] = transpose8x8(lo);
     }
@@ -237,9 +263,13 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
         mma_bf16_16816(o[nt][j], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
       }
     }
+    if (more) load_v(j0_next, pid);
   }
 
   // ---- the warps' shares of the split, in shared memory ----
+  // A lane holds, of each of its columns, 8 consecutive d (and 8 more 64 further on, 128 wide):
+  // 16-byte stores, the two halves in an order that keeps a quarter warp's on distinct banks.
+  constexpr int OS = D + 4;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -248,47 +278,64 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
 #pragma unroll
       for (int x = 4; x <= 16; x <<= 1) lv += __shfl_xor_sync(0xffffffffu, lv, x);
       const int r = 8 * nt + 2 * t + e;
-      if (g == 0) {
-        sm_m[warp][r] = m[nt][e];
-        sm_l[warp][r] = lv;
-      }
-      float* dst = sm_o + (warp * RT + r) * D;
+      if (g == 0) sm_ml[warp][r] = make_float2(m[nt][e], lv);
+      float* dst = sm_o + (warp * RT + r) * OS + 8 * g;
+      if (r < rows) {
 #pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        dst[8 * g + j] = o[nt][j][e];
-        dst[D == 128 ? 64 + 8 * g + j : 8 * g + j + 4] = o[nt][j][2 + e];
+        for (int c = 0; c < VC; ++c) {
+          const float4 v0 = make_float4(o[nt][0][2 * c + e], o[nt][1][2 * c + e], o[nt][2][2 * c + e], o[nt][3][2 * c + e]);
+          const float4 v1 = VC == 2 ? make_float4(o[nt][MT - 4][2 * c + e], o[nt][MT - 3][2 * c + e],
+                                                  o[nt][MT - 2][2 * c + e], o[nt][MT - 1][2 * c + e])
+                                    : make_float4(o[nt][0][2 + e], o[nt][1][2 + e], o[nt][2][2 + e], o[nt][3][2 + e]);
+          *reinterpret_cast<float4*>(dst + 64 * c + 4 * (t & 1)) = (t & 1) ? v1 : v0;
+          *reinterpret_cast<float4*>(dst + 64 * c + 4 * (t & 1 ^ 1)) = (t & 1) ? v0 : v1;
+        }
       }
     }
   __syncthreads();
-  const int pair = (b * a.Hkv + h) * a.tiles + tile;
-  float* part = a.part + ((size_t)pair * a.splits + split) * RT * (D + 2);
-  auto store = [&](int r, int d, float v) {
-    const Row q(a, h, r0 + r);
-    a.out[(((size_t)b * a.Lq + q.t) * a.Hq + q.head) * D + d] = f2bf(first + q.t >= 0 ? v : 0.f);
-  };
-  for (int i = threadIdx.x; i < rows * D; i += kWinThreads) {
-    const int r = i / D, d = i % D;
-    float M = -INFINITY;
+  if (threadIdx.x < rows) {  // the warps' weights in the split's sum, and its maximum and norm
+    const int r = threadIdx.x;
+    float M = -INFINITY, L = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWinWarps; ++w) M = fmaxf(M, sm_m[w][r]);
-    float L = 0.f, O = 0.f;
+    for (int w = 0; w < kWinWarps; ++w) M = fmaxf(M, sm_ml[w][r].x);
 #pragma unroll
     for (int w = 0; w < kWinWarps; ++w) {
-      const float f = sm_m[w][r] == -INFINITY ? 0.f : exp2f(sm_m[w][r] - M);
-      L = fmaf(f, sm_l[w][r], L);
-      O = fmaf(f, sm_o[(w * RT + r) * D + d], O);
+      const float f = M == -INFINITY ? 0.f : exp2f(sm_ml[w][r].x - M);
+      sm_f[w][r] = f;
+      L = fmaf(f, sm_ml[w][r].y, L);
     }
-    if (a.splits == 1) {
-      store(r, d, L > 0.f ? O / L : 0.f);
-    } else {
-      part[r * (D + 2) + d] = O;
-      if (d == 0) {
-        part[r * (D + 2) + D] = M;
-        part[r * (D + 2) + D + 1] = L;
-      }
+    sm_ml[0][r] = make_float2(M, L);
+  }
+  __syncthreads();
+  const int pair = (b * a.Hkv + h) * a.tiles + tile;
+  // row r, d .. d + 3 of the output (f: 1 / norm)
+  auto store = [&](int r, int d, float4 v, float f) {
+    const Row q(a, h, r0 + r);
+    // (a row without position may hold sums over other rows' keys)
+    const uint2 w = first + q.t < 0 ? make_uint2(0, 0) : make_uint2(pack_bf2(v.x * f, v.y * f), pack_bf2(v.z * f, v.w * f));
+    *reinterpret_cast<uint2*>(a.out + (((size_t)b * a.Lq + q.t) * a.Hq + q.head) * D + d) = w;
+  };
+  float* po = a.part + ((size_t)pair * a.splits + split) * RT * D;
+  float2* pml = a.part_ml + ((size_t)pair * a.splits + split) * RT;
+  for (int i = threadIdx.x; i < rows * (D / 4); i += kWinThreads) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4));
+    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWinWarps; ++w) {
+      const float f = sm_f[w][r];
+      const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * RT + r) * OS + d);
+      O.x = fmaf(f, v.x, O.x);
+      O.y = fmaf(f, v.y, O.y);
+      O.z = fmaf(f, v.z, O.z);
+      O.w = fmaf(f, v.w, O.w);
     }
+    if (a.splits == 1)
+      store(r, d, O, sm_ml[0][r].y > 0.f ? 1.f / sm_ml[0][r].y : 0.f);
+    else
+      *reinterpret_cast<float4*>(po + r * D + d) = O;
   }
   if (a.splits == 1) return;
+  if (threadIdx.x < rows) pml[threadIdx.x] = sm_ml[0][threadIdx.x];
 
   // ---- the last split to finish joins them, in the order of the splits ----
   __threadfence();
@@ -297,21 +344,44 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
   __syncthreads();
   if (!is_last) return;
   __threadfence();
-  const float* parts = a.part + (size_t)pair * a.splits * RT * (D + 2);
-  for (int i = threadIdx.x; i < rows * D; i += kWinThreads) {
-    const int r = i / D, d = i % D;
-    const float* p = parts + r * (D + 2);
-    float M = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, __ldcg(p + (size_t)s * RT * (D + 2) + D));
-    float L = 0.f, O = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-      const float* q = p + (size_t)s * RT * (D + 2);
-      const float ms = __ldcg(q + D);
-      const float f = ms == -INFINITY ? 0.f : exp2f(ms - M);
-      L = fmaf(f, __ldcg(q + D + 1), L);
-      O = fmaf(f, __ldcg(q + d), O);
+  const float* part = a.part + (size_t)pair * a.splits * RT * D;
+  const float2* part_ml = a.part_ml + (size_t)pair * a.splits * RT;
+  float* weight = sm_o;  // [rows][splits]: the splits' weights over the whole norm
+  for (int r = warp; r < rows; r += kWinWarps) {
+    float2 v[kMaxSplits / 32];
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMaxSplits / 32; ++i) {
+      const int s = lane + 32 * i;
+      v[i] = s < a.splits ? __ldcg(part_ml + (size_t)s * RT + r) : make_float2(-INFINITY, 0.f);
+      M = fmaxf(M, v[i].x);
     }
-    store(r, d, L > 0.f ? O / L : 0.f);
+    M = warp_max(M);
+#pragma unroll
+    for (int i = 0; i < kMaxSplits / 32; ++i) {
+      v[i].x = M == -INFINITY ? 0.f : exp2f(v[i].x - M);
+      L = fmaf(v[i].x, v[i].y, L);
+    }
+    L = warp_sum(L);
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+    for (int i = 0; i < kMaxSplits / 32; ++i)
+      if (lane + 32 * i < a.splits) weight[r * a.splits + lane + 32 * i] = v[i].x * inv;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * (D / 4); i += kWinThreads) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4));
+    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int s = 0; s < a.splits; ++s) {
+      const float f = weight[r * a.splits + s];
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(part + ((size_t)s * RT + r) * D + d));
+      O.x = fmaf(f, v.x, O.x);
+      O.y = fmaf(f, v.y, O.y);
+      O.z = fmaf(f, v.z, O.z);
+      O.w = fmaf(f, v.w, O.w);
+    }
+    store(r, d, O, 1.f);
   }
   if (threadIdx.x == 0) a.counters[pair] = 0;
 }
@@ -346,10 +416,14 @@ bool window_shape_ok(int B, int Lq, int Hq, int Hkv, int D, int max_seq_len, int
          B <= 65535;
 }
 
+// Above 64 query rows per kv head the 128-row tiles of the tcgen05 kernel (prefill_attn.cu) take
+// over, as they do for higgs_paged_attention.
+bool window_on_tc(int Lq, int Hq, int Hkv) { return prefill_attn_tc_on() && (int64_t)(Hq / Hkv) * Lq > 64; }
+
 template <int D, int NT>
 cudaError_t launch_window(const WinArgs& a, int B, cudaStream_t st) {
   auto k = window_decode_kernel<D, NT>;
-  const size_t smem = (size_t)kWinWarps * 8 * NT * D * sizeof(float);
+  const size_t smem = (size_t)kWinWarps * 8 * NT * (D + 4) * sizeof(float);
   static PerDeviceOnce attr;
   const cudaError_t e =
       attr.run([&] { return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); });
@@ -365,6 +439,9 @@ using namespace higgs;
 extern "C" size_t higgs_window_attention_workspace_size(int B, int Lq, int Hq, int Hkv, int D, int max_seq_len,
                                                         int window, int sinks) {
   if (!window_shape_ok(B, Lq, Hq, Hkv, D, max_seq_len, window, sinks)) return 0;
+  if (window_on_tc(Lq, Hq, Hkv)) return kWinCounterBytes;
+  window = std::min(window, max_seq_len);
+  sinks = std::min(sinks, max_seq_len);
   return window_ws_bytes(plan_window(B, Lq, Hq, Hkv, max_seq_len, window, sinks), B, Hkv, D);
 }
 
@@ -385,13 +462,25 @@ extern "C" int higgs_window_attention(higgs_ctx* ctx, const void* q, int B, int 
                 15) == 0 &&
                    page_stride % 8 == 0 && head_stride % 8 == 0,
                "higgs_window_attention: tensors, workspace and strides must be 16-byte aligned");
+  HG_CHECK_ARG(scale > 0.f && scale < INFINITY, "higgs_window_attention: scale must be positive and finite");
+  // a window or sinks past the longest sequence are the whole sequence
+  window = std::min(window, max_seq_len);
+  sinks = std::min(sinks, max_seq_len);
+  const bool tc = window_on_tc(Lq, Hq, Hkv);
   const WinPlan p = plan_window(B, Lq, Hq, Hkv, max_seq_len, window, sinks);
-  HG_CHECK_ARG((int64_t)Hkv * p.tiles <= 65535, "higgs_window_attention: too many query rows");
-  const size_t need = window_ws_bytes(p, B, Hkv, D);
+  HG_CHECK_ARG(tc ? (int64_t)B * Lq * Hq <= (1 << 30) : (int64_t)Hkv * p.tiles <= 65535,
+               "higgs_window_attention: too many query rows");
+  const size_t need = tc ? kWinCounterBytes : window_ws_bytes(p, B, Hkv, D);
   if (workspace_bytes < need)
     return fail(HIGGS_ERR_WORKSPACE,
                 "higgs_window_attention: workspace too small (need " + std::to_string(need) + " bytes)");
   HG_DEVICE(ctx);
+  if (tc) {
+    HG_CUDA(launch_prefill_attn_tc(q, B, Lq, Hq, Hkv, D, k_cache, v_cache, page_stride, head_stride, block_table,
+                                   max_blocks, seq_lens, scale, out, (int*)workspace, tc_err_ptr(),
+                                   (cudaStream_t)stream, window, sinks));
+    return HIGGS_OK;
+  }
   WinArgs a;
   a.q = (const uint16_t*)q;
   a.kc = (const uint16_t*)k_cache;
@@ -412,6 +501,7 @@ extern "C" int higgs_window_attention(higgs_ctx* ctx, const void* q, int B, int 
   a.tiles = p.tiles;
   a.counters = (int*)workspace;
   a.part = (float*)((char*)workspace + kWinCounterBytes);
+  a.part_ml = (float2*)(a.part + (size_t)B * Hkv * p.tiles * p.splits * 8 * p.nt * D);
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
   if (D == 64)

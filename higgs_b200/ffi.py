@@ -117,12 +117,6 @@ class ChainGemv(ctypes.Structure):
                 ("b2", P), ("y", P), ("y_f32", P), ("residual", P)]
 
 
-class KvPool(ctypes.Structure):
-    """higgs_kv_pool (include/higgs_cuda.h)."""
-    _fields_ = [("base", P), ("layers", I), ("num_pages", I64), ("layer_stride", I64),
-                ("page_stride", I64), ("page_bytes", I64)]
-
-
 class ModelConfig(ctypes.Structure):
     """higgs_model_config (include/higgs_cuda.h)."""
     _fields_ = [("hidden", I), ("layers", I), ("intermediate", I), ("heads", I), ("kv_heads", I),
@@ -177,7 +171,7 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
 
 
 def call(name: str, *args) -> int:
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != 0:
         raise HiggsError(name, rc, lib.higgs_last_error().decode())

@@ -23,7 +23,8 @@ def _p(t):
 
 
 def _st(dev: torch.device):
-    return torch.cuda.current_stream(dev).cuda_stream
+    """The device's current stream as a cudaStream_t (no Stream object is made)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if dev.index is None else dev.index)
 
 
 def _ctx(t: torch.Tensor) -> int:
@@ -39,10 +40,11 @@ def _chk(t: torch.Tensor, dtype, name: str):
         raise ValueError(f"{name} must be contiguous")
 
 
-def _same_device(x: torch.Tensor, **others):
-    for name, t in others.items():
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, not on {x.device}")
+def _same_device(x: torch.Tensor, *others):
+    dev = x.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on {x.device} and {t.device} in one call")
 
 
 # ---- a1/a2 ----------------------------------------------------------------
@@ -306,56 +308,68 @@ def window_attention(q, k_cache, v_cache, block_table, seq_lens, max_seq_len: in
     _chk(q, torch.bfloat16, "q")
     _chk(block_table, torch.int32, "block_table")
     _chk(seq_lens, torch.int32, "seq_lens")
-    if q.dim() != 4 or k_cache.dim() != 4:
+    if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16:
+        raise TypeError(f"the caches must be torch.bfloat16, got {k_cache.dtype} and {v_cache.dtype}")
+    shape, strides = k_cache.shape, k_cache.stride()
+    if q.dim() != 4 or len(shape) != 4:
         raise ValueError("q must be [B, Lq, Hq, D] and the caches [num_pages, Hkv, 16, D]")
     B, Lq, Hq, D = q.shape
-    Hkv = k_cache.shape[1]
-    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if c.dtype != torch.bfloat16:
-            raise TypeError(f"{name} must be torch.bfloat16, got {c.dtype}")
-        if c.shape != k_cache.shape or tuple(c.shape[2:]) != (PAGE, D):
-            raise ValueError(f"{name} must be [num_pages, Hkv, {PAGE}, {D}], got {list(c.shape)}")
-        if c.stride() != k_cache.stride() or c.stride()[2:] != (D, 1):
-            raise ValueError("the caches need equal strides and contiguous (page, head) blocks")
-    if block_table.dim() != 2 or block_table.shape[0] != B or tuple(seq_lens.shape) != (B,):
+    if shape[2] != PAGE or shape[3] != D or v_cache.shape != shape:
+        raise ValueError(f"the caches must be [num_pages, Hkv, {PAGE}, {D}], got {list(shape)} and "
+                         f"{list(v_cache.shape)}")
+    if v_cache.stride() != strides or strides[2] != D or strides[3] != 1:
+        raise ValueError("the caches need equal strides and contiguous (page, head) blocks")
+    if block_table.dim() != 2 or block_table.shape[0] != B or seq_lens.shape != (B,):
         raise ValueError("block_table must be [B, max_blocks] and seq_lens [B]")
     ctx = _ctx(q)
-    _same_device(q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, seq_lens=seq_lens,
-                 workspace=workspace)
+    _same_device(q, k_cache, v_cache, block_table, seq_lens, workspace)
+    Hkv = shape[1]
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     if workspace is None:
-        workspace = window_attention_workspace(B, Lq, Hq, Hkv, D, int(max_seq_len), int(window), int(sinks),
-                                               q.device)
+        workspace = window_attention_workspace(B, Lq, Hq, Hkv, D, max_seq_len, window, sinks, q.device)
     out = torch.empty_like(q)
-    ffi.call("higgs_window_attention", ctx, _p(q), B, Lq, Hq, Hkv, D, _p(k_cache), _p(v_cache),
-             k_cache.stride(0), k_cache.stride(1), _p(block_table), block_table.shape[1], _p(seq_lens),
-             int(max_seq_len), int(window), int(sinks), float(scale), _p(out), _p(workspace),
-             workspace.numel(), _st(q.device))
+    ffi.call("higgs_window_attention", ctx, q.data_ptr(), B, Lq, Hq, Hkv, D, k_cache.data_ptr(),
+             v_cache.data_ptr(), strides[0], strides[1], block_table.data_ptr(), block_table.shape[1],
+             seq_lens.data_ptr(), int(max_seq_len), int(window), int(sinks), float(scale), out.data_ptr(),
+             workspace.data_ptr(), workspace.numel(), _st(q.device))
     return out
+
+
+def _page_list(a) -> np.ndarray:
+    a = np.asarray(a)
+    if a.dtype != np.int32:
+        if a.size and (a.dtype.kind not in "iu" or int(a.max()) > 2 ** 31 - 1 or int(a.min()) < -2 ** 31):
+            raise ValueError("page lists must hold 32-bit whole numbers")
+        a = a.astype(np.int32)
+    return np.ascontiguousarray(a.reshape(-1))
 
 
 def kv_copy_pages(pools, src, dst) -> None:
     """In every tensor [layers, num_pages, ...] of ``pools`` and every layer of it, page dst[i]
     becomes page src[i]; see higgs_kv_copy_pages.  The tensors are a cache's K and V (or its codes
     and scales), each page contiguous; src and dst are host lists of page ids."""
-    pools = list(pools)
     if not pools:
         raise ValueError("kv_copy_pages: no pools")
-    src, dst = (np.ascontiguousarray(a, dtype=np.int32).reshape(-1) for a in (src, dst))
+    src, dst = _page_list(src), _page_list(dst)
     if src.size != dst.size:
         raise ValueError(f"kv_copy_pages: {src.size} sources, {dst.size} destinations")
-    arr = (ffi.KvPool * len(pools))()
-    for a, t in zip(arr, pools):
-        if t.dim() < 3 or not t[0, 0].is_contiguous():
+    words = []  # higgs_kv_pool: six 8-byte fields
+    for t in pools:
+        shape, strides, es = t.shape, t.stride(), t.element_size()
+        page = 1
+        for n, st in zip(reversed(shape[2:]), reversed(strides[2:])):
+            if n != 1 and st != page:
+                page = -1
+                break
+            page *= n
+        if len(shape) < 3 or page < 0:
             raise ValueError("a pool must be [layers, num_pages, ...] with contiguous pages")
-        _same_device(pools[0], pool=t)
-        es = t.element_size()
-        a.base, a.layers, a.num_pages = _p(t), t.shape[0], t.shape[1]
-        a.layer_stride, a.page_stride = t.stride(0) * es, t.stride(1) * es
-        a.page_bytes = math.prod(t.shape[2:]) * es
-    ffi.call("higgs_kv_copy_pages", _ctx(pools[0]), arr, len(pools), src.ctypes.data_as(ctypes.c_void_p),
-             dst.ctypes.data_as(ctypes.c_void_p), src.size, _st(pools[0].device))
+        words += (t.data_ptr(), shape[0], shape[1], strides[0] * es, strides[1] * es, page * es)
+    _same_device(*pools)
+    ffi.call("higgs_kv_copy_pages", _ctx(pools[0]), (ctypes.c_int64 * len(words))(*words), len(pools),
+             src.__array_interface__["data"][0], dst.__array_interface__["data"][0], src.size,
+             _st(pools[0].device))
 
 
 def tq4_encode(x, signs):
@@ -465,15 +479,16 @@ def beam_select(logits, scores, n_out: int, workspace=None):
     if logits.numel() != B * W * V:
         raise ValueError(f"logits must hold {B} x {W} rows, got {list(logits.shape)}")
     ctx = _ctx(logits)
-    _same_device(logits, scores=scores, workspace=workspace)
+    _same_device(logits, scores, workspace)
     if workspace is None:
-        workspace = beam_select_workspace(B, W, V, int(n_out), logits.device)
+        workspace = beam_select_workspace(B, W, V, n_out, logits.device)
     dev = logits.device
-    best = torch.empty(B, max(int(n_out), 0), dtype=torch.float32, device=dev)
-    beams = torch.empty(best.shape, dtype=torch.int32, device=dev)
-    tokens = torch.empty(best.shape, dtype=torch.int32, device=dev)
-    ffi.call("higgs_beam_select", ctx, _p(logits), _p(scores), B, W, V, int(n_out), _p(best), _p(beams),
-             _p(tokens), _p(workspace), workspace.numel(), _st(dev))
+    n_out = int(n_out)
+    best = torch.empty(B, max(n_out, 0), dtype=torch.float32, device=dev)
+    beams = torch.empty_like(best, dtype=torch.int32)
+    tokens = torch.empty_like(beams)
+    ffi.call("higgs_beam_select", ctx, logits.data_ptr(), scores.data_ptr(), B, W, V, n_out, best.data_ptr(),
+             beams.data_ptr(), tokens.data_ptr(), workspace.data_ptr(), workspace.numel(), _st(dev))
     return best, beams, tokens
 
 
