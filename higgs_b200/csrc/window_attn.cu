@@ -8,18 +8,23 @@
 // and give zeros.
 //
 // Decode kernel (few query rows per kv head).  A CTA takes a split of the visible pages of one
-// (sequence, kv head, tile of query rows = tokens x the G heads of the kv head), its 4 warps
-// alternate over the pages.  The page's 16 keys are the MMA's 16 rows and up to 8 query rows its
-// 8 columns, so G = 4 heads waste half of the tile and not three quarters of it:
+// (sequence, kv head, tile of 8 query rows = tokens x the G heads of the kv head), its 4 warps
+// alternate over the pages.  The page's 16 keys are the MMA's 16 rows and the query rows its 8
+// columns, so G = 4 heads waste half of the tile and not three quarters of it:
 //   S^T = K Q^T     A = K, 16 keys x 16 of d,     B = Q^T
 //   O^T += V^T P^T  A = V^T, 16 of d x 16 keys,   B = P^T
 // Both A operands come straight from global memory, 16 bytes per lane and load, with no shared
 // memory between: the sum over d may run in any order, so a lane's 16 bytes of a K row serve two
 // MMA steps (Q is laid out the same way); and the rows of O^T may be any d, so a lane loads 16
 // bytes of each of its 4 keys of V and pairs the keys with PRMT.  P^T goes from the accumulator's
-// layout to B's by an 8x8 transpose in registers (movmatrix), as bf16 hi + lo halves.  The running
-// maximum moves only when a score exceeds it by 2^kSlack.
-// Bound: HBM, 4 * D bytes per visible key and kv head.
+// layout to B's by an 8x8 transpose in registers (movmatrix), as bf16 hi + lo halves: 16 bits of
+// the weights, as in the other decode kernels.  The running maximum moves only when a score
+// exceeds it by 2^kSlack.  Tiles of 16 or 32 query rows (more columns per page load) measured
+// slower for six-token verifies, 8 sequences of 1000 visible keys 15.9 and 19.0 against 13.1 us:
+// the warps' chains get longer while the GPU is far from full.
+// Bound: HBM, 4 * D bytes per visible key and kv head.  B200, D = 128, 8 kv heads: 32 sequences of
+// 4100 visible keys (537 MB) 90.7 us = 5.93 TB/s, 0.92 of a copy; one sequence of 1028 keys 6.6 us,
+// bound by its chain of launch, length, page id, page, merge, counter and join.
 #include <algorithm>
 
 #include "common.cuh"
@@ -31,9 +36,9 @@ namespace {
 constexpr int kWinThreads = 128;
 constexpr int kWinWarps = kWinThreads / 32;
 constexpr int kWinCounterBytes = 16384;
+constexpr int kRows = 8;  // query rows of a tile: the columns of the MMA
 constexpr int kMaxSplits = 64;
-constexpr int kTargetCtas = 4 * 148;
-static_assert(kTargetCtas / 2 <= kWinCounterBytes / 4, "launches of two splits or more count in the workspace");
+constexpr int kCtasPerSm128 = 3, kCtasPerSm64 = 5;  // resident at once (registers)
 constexpr float kSlack = 8.0f;  // log2
 
 struct WinArgs {
@@ -44,7 +49,8 @@ struct WinArgs {
   const int32_t* bt;
   int max_blocks;
   const int32_t* seq_lens;
-  int Lq, Hq, Hkv, window, sinks;
+  int Lq, Hq, Hkv, G, window, sinks;
+  uint32_t inv_G;  // 2^32 / G, rounded up
   float scale_log2;
   uint16_t* out;
   int splits, tiles;
@@ -80,31 +86,38 @@ __device__ __forceinline__ uint4 ldg16_if(const uint16_t* p, bool ok) {
   return ok ? ldg_stream_u4(p) : make_uint4(0, 0, 0, 0);
 }
 
-// Row r of the tile as (query token, query head) of the call.
+// Row r of kv head h's tokens x heads as (query token, query head) of the call: r / G by a
+// multiplication (exact while r * G < 2^32, which the host checks).
 struct Row {
   int t, head;
   __device__ Row(const WinArgs& a, int h, int r) {
-    const int G = a.Hq / a.Hkv;
-    t = r / G;
-    head = h * G + r % G;
+    t = a.G == 1 ? r : (int)__umulhi((uint32_t)r, a.inv_G);
+    head = h * a.G + r - t * a.G;
   }
 };
 
-template <int D, int NT>
+// 2^x, results below 2^-126 flushed to zero
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int D>
 __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
-  constexpr int RT = 8 * NT;     // query rows of a tile
   constexpr int KC = D / 32;     // 16-byte chunks of a K row per lane
   constexpr int VC = D / 64;     // 16-byte chunks of a V row per lane
   constexpr int MT = D / 16;     // 16-row tiles of O^T
-  constexpr int QS = D + 8;      // padded row of Q in shared memory
-  __shared__ __align__(16) uint16_t qs[RT * QS];
-  __shared__ float2 sm_ml[kWinWarps][RT];  // maximum, norm
-  __shared__ float sm_f[kWinWarps][RT];
-  extern __shared__ __align__(16) float sm_o[];  // [warps][RT][D + 4]
+  constexpr int QS = D + 8;      // padded rows of Q and of O in shared memory
+  constexpr int OS = D + 4;
+  __shared__ __align__(16) uint16_t qs[kRows * QS];
+  __shared__ __align__(16) float sm_o[kWinWarps * kRows * OS];
+  __shared__ float2 sm_ml[kWinWarps][kRows];  // maximum, norm
+  __shared__ float sm_f[kWinWarps][kRows];
   __shared__ int is_last;
-  const int split = blockIdx.x, h = blockIdx.y / a.tiles, tile = blockIdx.y % a.tiles, b = blockIdx.z;
+  const int split = blockIdx.x, h = blockIdx.y / a.tiles, tile = blockIdx.y - h * a.tiles, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int R = (a.Hq / a.Hkv) * a.Lq, r0 = tile * RT, rows = min(RT, R - r0);
+  const int R = a.G * a.Lq, r0 = tile * kRows, rows = min(kRows, R - r0);
 
   pdl_wait();
   pdl_launch();
@@ -155,7 +168,7 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
   }
 
   // Q tile, rows past the last one zero
-  for (int i = threadIdx.x; i < RT * (D / 8); i += kWinThreads) {
+  for (int i = threadIdx.x; i < kRows * (D / 8); i += kWinThreads) {
     const int r = i / (D / 8), c = i % (D / 8);
     uint4 v = make_uint4(0, 0, 0, 0);
     if (r < rows) {
@@ -164,23 +177,22 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
     }
     *reinterpret_cast<uint4*>(qs + r * QS + c * 8) = v;
   }
-  int pos[NT][2];  // positions of this lane's columns 8 nt + 2 t + {0, 1}
-  float m[NT][2], l[NT][2], o[NT][MT][4];
+  int pos[2];  // positions of this lane's columns 2 t + {0, 1}
+  float m[2], l[2], o[MT][4];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = 8 * nt + 2 * t + e;
-      pos[nt][e] = r < rows ? first + Row(a, h, r0 + r).t : -1;
-      m[nt][e] = -INFINITY;
-      l[nt][e] = 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < MT; ++j)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) o[nt][j][c] = 0.f;
+  for (int e = 0; e < 2; ++e) {
+    pos[e] = 2 * t + e < rows ? first + Row(a, h, r0 + 2 * t + e).t : -1;
+    m[e] = -INFINITY;
+    l[e] = 0.f;
   }
+#pragma unroll
+  for (int j = 0; j < MT; ++j)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[j][c] = 0.f;
   __syncthreads();
+  uint4 qf[KC];  // Q^T fragments
+#pragma unroll
+  for (int i = 0; i < KC; ++i) qf[i] = *reinterpret_cast<const uint4*>(qs + g * QS + (4 * i + t) * 8);
 
   for (; u < u1; u += kWinWarps) {
     const int j0 = vis.page(u) * 16;
@@ -188,66 +200,57 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
     const int j0_next = more ? vis.page(u + kWinWarps) * 16 : 0;
     pid = pid_next;
     if (u + 2 * kWinWarps < u1) pid_next = bt[vis.page(u + 2 * kWinWarps)];
-    float s[NT][4];  // (key g, column 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1)
+    // (key g, column 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1); two chains of products
+    float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) s[nt][c] = 0.f;
-#pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        const uint4 qv = *reinterpret_cast<const uint4*>(qs + (8 * nt + g) * QS + (4 * i + t) * 8);
-        mma_bf16_16816(s[nt], kf[0][i].x, kf[1][i].x, kf[0][i].y, kf[1][i].y, qv.x, qv.y);
-        mma_bf16_16816(s[nt], kf[0][i].z, kf[1][i].z, kf[0][i].w, kf[1][i].w, qv.z, qv.w);
-      }
+    for (int i = 0; i < KC; ++i) {
+      mma_bf16_16816(s, kf[0][i].x, kf[1][i].x, kf[0][i].y, kf[1][i].y, qf[i].x, qf[i].y);
+      mma_bf16_16816(s2, kf[0][i].z, kf[1][i].z, kf[0][i].w, kf[1][i].w, qf[i].z, qf[i].w);
     }
     if (more) load_k(j0_next, pid);
-    uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int c = 0; c < 4; ++c) s[c] = (s[c] + s2[c]) * a.scale_log2;
+    if (!in) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) s[nt][c] *= a.scale_log2;
-      if (!in) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int j = j0 + g + 8 * (c >> 1), p = pos[nt][c & 1];
-          if (!(j <= p && (j > p - a.window || j < a.sinks))) s[nt][c] = -INFINITY;
-        }
+      for (int c = 0; c < 4; ++c) {
+        const int j = j0 + g + 8 * (c >> 1), p = pos[c & 1];
+        if (!(j <= p && (j > p - a.window || j < a.sinks))) s[c] = -INFINITY;
       }
-      float mx[2] = {fmaxf(s[nt][0], s[nt][2]), fmaxf(s[nt][1], s[nt][3])};
-      if (__any_sync(0xffffffffu, mx[0] > m[nt][0] + kSlack || mx[1] > m[nt][1] + kSlack)) {
-        float alpha[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-          for (int x = 4; x <= 16; x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
-          const float mn = fmaxf(m[nt][e], mx[e]);
-          alpha[e] = mn == -INFINITY ? 1.f : exp2f(m[nt][e] - mn);
-          m[nt][e] = mn;
-          l[nt][e] *= alpha[e];
-        }
-#pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          o[nt][j][0] *= alpha[0];
-          o[nt][j][1] *= alpha[1];
-          o[nt][j][2] *= alpha[0];
-          o[nt][j][3] *= alpha[1];
-        }
-      }
-      const float b0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], b1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
-      s[nt][0] = exp2f(s[nt][0] - b0);
-      s[nt][1] = exp2f(s[nt][1] - b1);
-      s[nt][2] = exp2f(s[nt][2] - b0);
-      s[nt][3] = exp2f(s[nt][3] - b1);
-      l[nt][0] += s[nt][0] + s[nt][2];
-      l[nt][1] += s[nt][1] + s[nt][3];
-      uint32_t hi, lo;
-      split_bf2(s[nt][0], s[nt][1], hi, lo);
-      ph[nt][0] = transpose8x8(hi);
-      pl[nt][0] = transpose8x8(lo);
-      split_bf2(s[nt][2], s[nt][3], hi, lo);
-      ph[nt][1] = transpose8x8(hi);
-      pl[nt][1] = transpose8x8(lo);
     }
+    float mx[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
+    if (__any_sync(0xffffffffu, mx[0] > m[0] + kSlack || mx[1] > m[1] + kSlack)) {
+      float alpha[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int x = 4; x <= 16; x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
+        const float mn = fmaxf(m[e], mx[e]);
+        alpha[e] = mn == -INFINITY ? 1.f : ex2(m[e] - mn);
+        m[e] = mn;
+        l[e] *= alpha[e];
+      }
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        o[j][0] *= alpha[0];
+        o[j][1] *= alpha[1];
+        o[j][2] *= alpha[0];
+        o[j][3] *= alpha[1];
+      }
+    }
+    const float b0 = m[0] == -INFINITY ? 0.f : m[0], b1 = m[1] == -INFINITY ? 0.f : m[1];
+    s[0] = ex2(s[0] - b0);
+    s[1] = ex2(s[1] - b1);
+    s[2] = ex2(s[2] - b0);
+    s[3] = ex2(s[3] - b1);
+    l[0] += s[0] + s[2];
+    l[1] += s[1] + s[3];
+    uint32_t hi0, lo0, hi1, lo1;
+    split_bf2(s[0], s[1], hi0, lo0);
+    split_bf2(s[2], s[3], hi1, lo1);
+    hi0 = transpose8x8(hi0);
+    hi1 = transpose8x8(hi1);
+    lo0 = transpose8x8(lo0);
+    lo1 = transpose8x8(lo1);
     // O^T tile j: rows g and g + 8 are d = 8 g + j and, 128 wide, 64 + 8 g + j; 64 wide, 8 g + j + 4
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
@@ -257,11 +260,8 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
       const uint32_t a1 = prmt(part4(vf[0][c1], e1 >> 1), part4(vf[1][c1], e1 >> 1), sel1);
       const uint32_t a2 = prmt(part4(vf[2][0], j >> 1), part4(vf[3][0], j >> 1), sel0);
       const uint32_t a3 = prmt(part4(vf[2][c1], e1 >> 1), part4(vf[3][c1], e1 >> 1), sel1);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        mma_bf16_16816(o[nt][j], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
-        mma_bf16_16816(o[nt][j], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
-      }
+      mma_bf16_16816(o[j], a0, a1, a2, a3, hi0, hi1);
+      mma_bf16_16816(o[j], a0, a1, a2, a3, lo0, lo1);
     }
     if (more) load_v(j0_next, pid);
   }
@@ -269,29 +269,25 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
   // ---- the warps' shares of the split, in shared memory ----
   // A lane holds, of each of its columns, 8 consecutive d (and 8 more 64 further on, 128 wide):
   // 16-byte stores, the two halves in an order that keeps a quarter warp's on distinct banks.
-  constexpr int OS = D + 4;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int e = 0; e < 2; ++e) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float lv = l[nt][e];
+    for (int x = 4; x <= 16; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
+    const int r = 2 * t + e;
+    if (g == 0) sm_ml[warp][r] = make_float2(m[e], l[e]);
+    float* dst = sm_o + (warp * kRows + r) * OS + 8 * g;
+    if (r < rows) {
 #pragma unroll
-      for (int x = 4; x <= 16; x <<= 1) lv += __shfl_xor_sync(0xffffffffu, lv, x);
-      const int r = 8 * nt + 2 * t + e;
-      if (g == 0) sm_ml[warp][r] = make_float2(m[nt][e], lv);
-      float* dst = sm_o + (warp * RT + r) * OS + 8 * g;
-      if (r < rows) {
-#pragma unroll
-        for (int c = 0; c < VC; ++c) {
-          const float4 v0 = make_float4(o[nt][0][2 * c + e], o[nt][1][2 * c + e], o[nt][2][2 * c + e], o[nt][3][2 * c + e]);
-          const float4 v1 = VC == 2 ? make_float4(o[nt][MT - 4][2 * c + e], o[nt][MT - 3][2 * c + e],
-                                                  o[nt][MT - 2][2 * c + e], o[nt][MT - 1][2 * c + e])
-                                    : make_float4(o[nt][0][2 + e], o[nt][1][2 + e], o[nt][2][2 + e], o[nt][3][2 + e]);
-          *reinterpret_cast<float4*>(dst + 64 * c + 4 * (t & 1)) = (t & 1) ? v1 : v0;
-          *reinterpret_cast<float4*>(dst + 64 * c + 4 * (t & 1 ^ 1)) = (t & 1) ? v0 : v1;
-        }
+      for (int c = 0; c < VC; ++c) {
+        // 128 wide: d = 64 c + 8 g + 0..7 in tiles 0..7; 64 wide: tiles 0..3, upper rows second
+        const int f = 2 * c + e, f2 = VC == 2 ? f : e + 2, j2 = VC == 2 ? 4 : 0;
+        const float4 v0 = make_float4(o[0][f], o[1][f], o[2][f], o[3][f]);
+        const float4 v1 = make_float4(o[j2][f2], o[j2 + 1][f2], o[j2 + 2][f2], o[j2 + 3][f2]);
+        *reinterpret_cast<float4*>(dst + 64 * c + 4 * (t & 1)) = (t & 1) ? v1 : v0;
+        *reinterpret_cast<float4*>(dst + 64 * c + 4 * ((t & 1) ^ 1)) = (t & 1) ? v0 : v1;
       }
     }
+  }
   __syncthreads();
   if (threadIdx.x < rows) {  // the warps' weights in the split's sum, and its maximum and norm
     const int r = threadIdx.x;
@@ -300,7 +296,7 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
     for (int w = 0; w < kWinWarps; ++w) M = fmaxf(M, sm_ml[w][r].x);
 #pragma unroll
     for (int w = 0; w < kWinWarps; ++w) {
-      const float f = M == -INFINITY ? 0.f : exp2f(sm_ml[w][r].x - M);
+      const float f = M == -INFINITY ? 0.f : ex2(sm_ml[w][r].x - M);
       sm_f[w][r] = f;
       L = fmaf(f, sm_ml[w][r].y, L);
     }
@@ -315,15 +311,15 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
     const uint2 w = first + q.t < 0 ? make_uint2(0, 0) : make_uint2(pack_bf2(v.x * f, v.y * f), pack_bf2(v.z * f, v.w * f));
     *reinterpret_cast<uint2*>(a.out + (((size_t)b * a.Lq + q.t) * a.Hq + q.head) * D + d) = w;
   };
-  float* po = a.part + ((size_t)pair * a.splits + split) * RT * D;
-  float2* pml = a.part_ml + ((size_t)pair * a.splits + split) * RT;
+  float* po = a.part + ((size_t)pair * a.splits + split) * kRows * D;
+  float2* pml = a.part_ml + ((size_t)pair * a.splits + split) * kRows;
   for (int i = threadIdx.x; i < rows * (D / 4); i += kWinThreads) {
     const int r = i / (D / 4), d = 4 * (i % (D / 4));
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWinWarps; ++w) {
       const float f = sm_f[w][r];
-      const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * RT + r) * OS + d);
+      const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * kRows + r) * OS + d);
       O.x = fmaf(f, v.x, O.x);
       O.y = fmaf(f, v.y, O.y);
       O.z = fmaf(f, v.z, O.z);
@@ -344,8 +340,8 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
   __syncthreads();
   if (!is_last) return;
   __threadfence();
-  const float* part = a.part + (size_t)pair * a.splits * RT * D;
-  const float2* part_ml = a.part_ml + (size_t)pair * a.splits * RT;
+  const float* part = a.part + (size_t)pair * a.splits * kRows * D;
+  const float2* part_ml = a.part_ml + (size_t)pair * a.splits * kRows;
   float* weight = sm_o;  // [rows][splits]: the splits' weights over the whole norm
   for (int r = warp; r < rows; r += kWinWarps) {
     float2 v[kMaxSplits / 32];
@@ -353,13 +349,13 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
 #pragma unroll
     for (int i = 0; i < kMaxSplits / 32; ++i) {
       const int s = lane + 32 * i;
-      v[i] = s < a.splits ? __ldcg(part_ml + (size_t)s * RT + r) : make_float2(-INFINITY, 0.f);
+      v[i] = s < a.splits ? __ldcg(part_ml + (size_t)s * kRows + r) : make_float2(-INFINITY, 0.f);
       M = fmaxf(M, v[i].x);
     }
     M = warp_max(M);
 #pragma unroll
     for (int i = 0; i < kMaxSplits / 32; ++i) {
-      v[i].x = M == -INFINITY ? 0.f : exp2f(v[i].x - M);
+      v[i].x = M == -INFINITY ? 0.f : ex2(v[i].x - M);
       L = fmaf(v[i].x, v[i].y, L);
     }
     L = warp_sum(L);
@@ -375,7 +371,7 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
 #pragma unroll 8
     for (int s = 0; s < a.splits; ++s) {
       const float f = weight[r * a.splits + s];
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(part + ((size_t)s * RT + r) * D + d));
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(part + ((size_t)s * kRows + r) * D + d));
       O.x = fmaf(f, v.x, O.x);
       O.y = fmaf(f, v.y, O.y);
       O.z = fmaf(f, v.z, O.z);
@@ -387,27 +383,34 @@ __global__ void __launch_bounds__(kWinThreads) window_decode_kernel(WinArgs a) {
 }
 
 struct WinPlan {
-  int nt, tiles, splits;
+  int tiles, splits;
 };
 
-// Row tiles of 8, 16 or 32 query rows; splits of the longest visible range so that the CTAs fill
-// the GPU, four pages (one per warp) at least.
-WinPlan plan_window(int B, int Lq, int Hq, int Hkv, int max_seq_len, int window, int sinks) {
+// Splits of the visible pages.  A CTA's time is its pages (4 warps) plus about four pages' worth
+// of start, merge and store; the splits that need the least over the waves of resident CTAs.
+WinPlan plan_window(int B, int Lq, int Hq, int Hkv, int D, int max_seq_len, int window, int sinks) {
   WinPlan p;
-  const int R = (Hq / Hkv) * Lq;
-  p.nt = R <= 8 ? 1 : R <= 16 ? 2 : 4;
-  p.tiles = (R + 8 * p.nt - 1) / (8 * p.nt);
-  const int64_t keys = std::min<int64_t>(max_seq_len, (int64_t)window + Lq + sinks);
-  const int pages = (int)std::min<int64_t>((max_seq_len + 15) / 16, (keys + 15) / 16 + 2);
-  const int64_t pairs = (int64_t)B * Hkv * p.tiles;
-  const int64_t want = std::max<int64_t>(1, kTargetCtas / pairs);
-  p.splits = (int)std::min<int64_t>(std::min<int64_t>(want, kMaxSplits), std::max(1, (pages + 3) / 4));
+  p.tiles = ((Hq / Hkv) * Lq + kRows - 1) / kRows;
+  const int64_t keys = std::min<int64_t>(max_seq_len, (int64_t)window + sinks + Lq);
+  const int64_t pages = std::min<int64_t>((max_seq_len + 15) / 16, (keys + 15) / 16 + 1);
+  const int64_t pairs = (int64_t)B * Hkv * p.tiles, slots = 148 * (D == 64 ? kCtasPerSm64 : kCtasPerSm128);
+  int64_t best = INT64_MAX;
+  p.splits = 1;
+  for (int s = 1; s <= std::min<int64_t>(kMaxSplits, (pages + kWinWarps - 1) / kWinWarps); ++s) {
+    if (s > 1 && pairs > kWinCounterBytes / 4) break;
+    const int64_t waves = (pairs * s + slots - 1) / slots;
+    const int64_t cost = waves * ((pages + (int64_t)kWinWarps * s - 1) / (kWinWarps * s) + 4);
+    if (cost < best) {
+      best = cost;
+      p.splits = s;
+    }
+  }
   return p;
 }
 
 size_t window_ws_bytes(const WinPlan& p, int B, int Hkv, int D) {
   if (p.splits == 1) return kWinCounterBytes;
-  return kWinCounterBytes + (size_t)B * Hkv * p.tiles * p.splits * 8 * p.nt * (D + 2) * sizeof(float);
+  return kWinCounterBytes + (size_t)B * Hkv * p.tiles * p.splits * kRows * (D + 2) * sizeof(float);
 }
 
 bool window_shape_ok(int B, int Lq, int Hq, int Hkv, int D, int max_seq_len, int window, int sinks) {
@@ -420,17 +423,6 @@ bool window_shape_ok(int B, int Lq, int Hq, int Hkv, int D, int max_seq_len, int
 // over, as they do for higgs_paged_attention.
 bool window_on_tc(int Lq, int Hq, int Hkv) { return prefill_attn_tc_on() && (int64_t)(Hq / Hkv) * Lq > 64; }
 
-template <int D, int NT>
-cudaError_t launch_window(const WinArgs& a, int B, cudaStream_t st) {
-  auto k = window_decode_kernel<D, NT>;
-  const size_t smem = (size_t)kWinWarps * 8 * NT * (D + 4) * sizeof(float);
-  static PerDeviceOnce attr;
-  const cudaError_t e =
-      attr.run([&] { return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); });
-  if (e != cudaSuccess) return e;
-  return launch_pdl(k, dim3(a.splits, a.Hkv * a.tiles, B), dim3(kWinThreads), smem, st, a);
-}
-
 }  // namespace
 }  // namespace higgs
 
@@ -442,7 +434,7 @@ extern "C" size_t higgs_window_attention_workspace_size(int B, int Lq, int Hq, i
   if (window_on_tc(Lq, Hq, Hkv)) return kWinCounterBytes;
   window = std::min(window, max_seq_len);
   sinks = std::min(sinks, max_seq_len);
-  return window_ws_bytes(plan_window(B, Lq, Hq, Hkv, max_seq_len, window, sinks), B, Hkv, D);
+  return window_ws_bytes(plan_window(B, Lq, Hq, Hkv, D, max_seq_len, window, sinks), B, Hkv, D);
 }
 
 extern "C" int higgs_window_attention(higgs_ctx* ctx, const void* q, int B, int Lq, int Hq, int Hkv, int D,
@@ -467,8 +459,9 @@ extern "C" int higgs_window_attention(higgs_ctx* ctx, const void* q, int B, int 
   window = std::min(window, max_seq_len);
   sinks = std::min(sinks, max_seq_len);
   const bool tc = window_on_tc(Lq, Hq, Hkv);
-  const WinPlan p = plan_window(B, Lq, Hq, Hkv, max_seq_len, window, sinks);
-  HG_CHECK_ARG(tc ? (int64_t)B * Lq * Hq <= (1 << 30) : (int64_t)Hkv * p.tiles <= 65535,
+  const WinPlan p = plan_window(B, Lq, Hq, Hkv, D, max_seq_len, window, sinks);
+  HG_CHECK_ARG(tc ? (int64_t)B * Lq * Hq <= (1 << 30)
+                  : (int64_t)Hkv * p.tiles <= 65535 && (int64_t)Lq * (Hq / Hkv) * (Hq / Hkv) < ((int64_t)1 << 32),
                "higgs_window_attention: too many query rows");
   const size_t need = tc ? kWinCounterBytes : window_ws_bytes(p, B, Hkv, D);
   if (workspace_bytes < need)
@@ -493,6 +486,8 @@ extern "C" int higgs_window_attention(higgs_ctx* ctx, const void* q, int B, int 
   a.Lq = Lq;
   a.Hq = Hq;
   a.Hkv = Hkv;
+  a.G = Hq / Hkv;
+  a.inv_G = (uint32_t)((((uint64_t)1 << 32) + a.G - 1) / a.G);
   a.window = window;
   a.sinks = sinks;
   a.scale_log2 = scale * 1.4426950408889634f;
@@ -501,15 +496,9 @@ extern "C" int higgs_window_attention(higgs_ctx* ctx, const void* q, int B, int 
   a.tiles = p.tiles;
   a.counters = (int*)workspace;
   a.part = (float*)((char*)workspace + kWinCounterBytes);
-  a.part_ml = (float2*)(a.part + (size_t)B * Hkv * p.tiles * p.splits * 8 * p.nt * D);
+  a.part_ml = (float2*)(a.part + (size_t)B * Hkv * p.tiles * p.splits * kRows * D);
   cudaStream_t st = (cudaStream_t)stream;
-  cudaError_t e;
-  if (D == 64)
-    e = p.nt == 1 ? launch_window<64, 1>(a, B, st) : p.nt == 2 ? launch_window<64, 2>(a, B, st)
-                                                               : launch_window<64, 4>(a, B, st);
-  else
-    e = p.nt == 1 ? launch_window<128, 1>(a, B, st) : p.nt == 2 ? launch_window<128, 2>(a, B, st)
-                                                                : launch_window<128, 4>(a, B, st);
-  HG_CUDA(e);
+  HG_CUDA(launch_pdl(D == 64 ? window_decode_kernel<64> : window_decode_kernel<128>,
+                     dim3(p.splits, Hkv * p.tiles, B), dim3(kWinThreads), 0, st, a));
   return HIGGS_OK;
 }
