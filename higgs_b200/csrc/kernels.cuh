@@ -216,8 +216,14 @@ bool prefill_attn_tc_fits(int Lq, int Hq, int Hkv, int D, const void* q, const v
 cudaError_t launch_prefill_attn_tc(const void* q, int B, int Lq, int Hq, int Hkv, int D, const void* kc,
                                    const void* vc, int64_t page_stride, int64_t head_stride, const int32_t* bt,
                                    int max_blocks, const int32_t* seq_lens, float scale, void* out, int* counters,
-                                   int* err, cudaStream_t st, int window = 0, int sinks = 0);
+                                   int* err, cudaStream_t st);
 bool prefill_attn_tc_on();
+
+// attention through a window with sinks above 64 query rows per kv head (window_prefill.cu)
+cudaError_t launch_window_prefill(const void* q, int B, int Lq, int Hq, int Hkv, int D, const void* kc, const void* vc,
+                                  int64_t page_stride, int64_t head_stride, const int32_t* bt, int max_blocks,
+                                  const int32_t* seq_lens, int window, int sinks, float scale, void* out,
+                                  int* counters, int* err, cudaStream_t st);
 int* tc_err_ptr();
 
 }  // namespace higgs

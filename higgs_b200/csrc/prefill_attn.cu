@@ -67,7 +67,6 @@ struct PfArgs {
   int max_blocks;
   const int32_t* seq_lens;
   int B, Lq, Hq, Hkv;
-  int window, sinks;  // WIN kernels only
   float scale_log2;
   uint16_t* out;
   int* err;
@@ -136,41 +135,16 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
 }
 
 // Tile i of a launch: query tile nqt - 1 - i / (B Hkv) (the longest causal ranges first) of
-// (sequence, kv head) i % (B Hkv).  Its 128-key blocks are the keys 0 .. kv_len - 1; with a window
-// (WIN), `sink_blocks` blocks from key 0 for the first `sink_keys` keys and then the blocks from
-// `base`, the page that holds the first key `lo` of the window of the tile's first token.
+// (sequence, kv head) i % (B Hkv)
 struct PfTile {
   int b, hkv, t0, t_end, pos0, kv_len, nkb;
-  int lo, base, sink_keys, sink_blocks;
 };
-// Rows of a tile: TQ = 128 / G tokens x G heads.  With a window rows are cut from the flat list of
-// tokens x heads instead, so that G need not divide 128.
-template <bool WIN>
-__device__ __forceinline__ int pf_num_qtiles(const PfArgs& a) {
-  const int G = a.Hq / a.Hkv;
-  if (WIN) return (a.Lq * G + kPfRows - 1) / kPfRows;
-  const int TQ = kPfRows / G;
-  return (a.Lq + TQ - 1) / TQ;
-}
-template <bool WIN>
 __device__ __forceinline__ PfTile pf_tile(const PfArgs& a, int i, int nqt) {
   PfTile T;
-  const int G = a.Hq / a.Hkv, TQ = kPfRows / G, bh = a.B * a.Hkv;
+  const int TQ = kPfRows / (a.Hq / a.Hkv), bh = a.B * a.Hkv;
   const int qt = nqt - 1 - i / bh;
   T.b = (i % bh) / a.Hkv;
   T.hkv = i % a.Hkv;
-  if (WIN) {
-    T.t0 = qt * kPfRows;  // first row
-    T.t_end = min(a.Lq * G, T.t0 + kPfRows);
-    T.pos0 = a.seq_lens[T.b] - a.Lq;
-    T.kv_len = max(0, min(T.pos0 + (T.t_end - 1) / G + 1, a.max_blocks * 16));
-    T.lo = max(0, max(0, T.pos0 + T.t0 / G) - a.window + 1);
-    T.base = T.lo & ~15;
-    T.sink_keys = min(a.sinks, T.base);
-    T.sink_blocks = T.kv_len > 0 ? (T.sink_keys + kPfKeys - 1) / kPfKeys : 0;
-    T.nkb = T.kv_len > 0 ? T.sink_blocks + (T.kv_len - T.base + kPfKeys - 1) / kPfKeys : 0;
-    return T;
-  }
   T.t0 = qt * TQ;
   T.t_end = min(a.Lq, T.t0 + TQ);              // the tile's tokens [t0, t_end)
   T.pos0 = a.seq_lens[T.b] - a.Lq;             // position of query token 0
@@ -185,7 +159,7 @@ __device__ __forceinline__ void pf_loaders_sync() {
   asm volatile("bar.sync 5, %0;" ::"n"(kPfLoaders) : "memory");
 }
 
-template <int D, bool WIN>
+template <int D>
 __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_tc_kernel(PfArgs a) {
   constexpr int S = pf_stages(D);
   constexpr uint32_t kQ = pf_q_bytes(D), kKV = pf_kv_bytes(D);
@@ -221,8 +195,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_tc_kernel(PfArgs a
   __shared__ int abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int G = a.Hq / a.Hkv;
-  const int nqt = pf_num_qtiles<WIN>(a);
+  const int G = a.Hq / a.Hkv, TQ = kPfRows / G;
+  const int nqt = (a.Lq + TQ - 1) / TQ;
   const int ntiles = nqt * a.B * a.Hkv;
   volatile int* abort = &abort_flag;
 
@@ -292,15 +266,15 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_tc_kernel(PfArgs a
       const int i = loader_tile;
       pf_loaders_sync();  // every loader has read it before the next round's write
       if (i >= ntiles) break;
-      const PfTile T = pf_tile<WIN>(a, i, nqt);
+      const PfTile T = pf_tile(a, i, nqt);
       // Q row r = (token t0 + r / G, query head hkv G + r % G), once the previous tile's
       // S MMAs are done with the buffer
       if (k >= 1) pf_wait(&q_empty, (k - 1) & 1, abort, a.err);
       for (int e = lt; e < kPfRows * DC; e += kPfLoaders) {
         const int r = e / DC, c = e % DC;
-        const int t = WIN ? (T.t0 + r) / G : T.t0 + r / G, hd = WIN ? (T.t0 + r) % G : r % G;
-        const bool ok = WIN ? T.t0 + r < T.t_end : t < T.t_end;
-        const uint16_t* src = a.q + (((size_t)T.b * a.Lq + (ok ? t : 0)) * a.Hq + T.hkv * G + hd) * D + c * 8;
+        const int t = T.t0 + r / G;
+        const bool ok = t < T.t_end;
+        const uint16_t* src = a.q + (((size_t)T.b * a.Lq + (ok ? t : 0)) * a.Hq + T.hkv * G + r % G) * D + c * 8;
         cp_async16_zfill(qs + (c >> 3) * (kPfRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src, ok);
       }
       cp_async_commit();
@@ -314,20 +288,15 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_tc_kernel(PfArgs a
         if (J >= S) pf_wait(&kv_empty[s], ((J / S) - 1) & 1, abort, a.err);
         uint8_t* ks = kvs + (size_t)s * 2 * kKV;
         uint8_t* vs = ks + kKV;
-        const bool sink_block = WIN && j < T.sink_blocks;
-        const int kb = WIN && !sink_block ? T.base + (j - T.sink_blocks) * kPfKeys : j * kPfKeys;
         int pg[KPT];
 #pragma unroll
         for (int q = 0; q < KPT; ++q) {
-          const int kg = kb + k0 + q * KSTEP;
-          bool ok = kg < T.kv_len;
-          // keys no query of the tile sees are not looked up: their page may be free
-          if (WIN) ok = sink_block ? kg < T.sink_keys : ok && (kg >= T.lo || kg < a.sinks);
-          pg[q] = ok ? btr[kg >> 4] : -1;
+          const int kg = j * kPfKeys + k0 + q * KSTEP;
+          pg[q] = kg < T.kv_len ? btr[kg >> 4] : -1;
         }
 #pragma unroll
         for (int q = 0; q < KPT; ++q) {
-          const int kg = kb + k0 + q * KSTEP;
+          const int kg = j * kPfKeys + k0 + q * KSTEP;
           const size_t off = pg[q] >= 0 ? (size_t)pg[q] * a.page_stride + col + (size_t)(kg & 15) * D : 0;
           const uint32_t so = so0 + (k0 + q * KSTEP) * 128;
           cp_async16_zfill(ks + so, a.kc + off, pg[q] >= 0);
@@ -359,7 +328,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_tc_kernel(PfArgs a
       for (int k = 0;; ++k) {
         const int i = next_tile(k);
         if (i >= ntiles) break;
-        const PfTile T = pf_tile<WIN>(a, i, nqt);
+        const PfTile T = pf_tile(a, i, nqt);
         pf_wait(&q_full, k & 1, abort, a.err);
         for (int j = 0; j < T.nkb; ++j, ++J) {
           const int s = J % S, sb = J & 1;
@@ -385,7 +354,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_tc_kernel(PfArgs a
       for (int k = 0;; ++k) {
         const int i = next_tile(k);
         if (i >= ntiles) break;
-        const PfTile T = pf_tile<WIN>(a, i, nqt);
+        const PfTile T = pf_tile(a, i, nqt);
         for (int j = 0; j < T.nkb; ++j, ++J) {
           const int s = J % S;
           // a tile's first P V overwrites O: the softmax threads have read the previous tile's
@@ -414,9 +383,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_tc_kernel(PfArgs a
     for (int k = 0;; ++k) {
       const int i = next_tile(k);
       if (i >= ntiles) break;
-      const PfTile T = pf_tile<WIN>(a, i, nqt);
-      const int t = WIN ? (T.t0 + r) / G : T.t0 + r / G, hd = WIN ? (T.t0 + r) % G : r % G;
-      const bool valid = WIN ? T.t0 + r < T.t_end : t < T.t_end;
+      const PfTile T = pf_tile(a, i, nqt);
+      const int t = T.t0 + r / G;
+      const bool valid = t < T.t_end;
       const int pos = valid ? T.pos0 + t : -1;  // keys 0 .. pos are visible
       float m = -INFINITY, l = 0.f;             // l: this half's share of the row sum
       for (int j = 0; j < T.nkb; ++j, ++J) {
@@ -429,27 +398,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_tc_kernel(PfArgs a
         tc_wait_ld();
         tc_fence_before();
         mbar_arrive(&s_free[sb]);  // S buffer sb may take S_{J+2}
-        const bool sink_block = WIN && j < T.sink_blocks;
-        const int kb = WIN && !sink_block ? T.base + (j - T.sink_blocks) * kPfKeys : j * kPfKeys;
-        int lim = pos - kb - hf * HK;  // key i of this half is visible iff i <= lim
-        // ... and, with a window, i >= low or i < snk
-        const int low = WIN ? pos - a.window + 1 - kb - hf * HK : 0, snk = WIN ? a.sinks - kb - hf * HK : 0;
-        if (sink_block) lim = min(lim, T.sink_keys - 1 - kb - hf * HK);
+        const int lim = pos - j * kPfKeys - hf * HK;  // key i of this half is visible iff i <= lim
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (lim >= HK - 1 && (!WIN || low <= 0 || snk >= HK)) {  // every key of this half visible: no mask
+        if (lim >= HK - 1) {  // every key of this half visible: no mask
 #pragma unroll
           for (int q = 0; q < HK; ++q) mx4[q & 3] = fmaxf(mx4[q & 3], v[q]);
-        } else if (WIN) {
-          // the visible keys as bits: (keys up to lim) and (keys from low on, or before snk)
-          auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
-          static_assert(HK == 64, "one bit per key of a half");
-          const unsigned long long vis = below(lim + 1) & (~below(low) | below(snk));
-          const uint32_t vb[2] = {(uint32_t)vis, (uint32_t)(vis >> 32)};
-#pragma unroll
-          for (int q = 0; q < HK; ++q) {
-            v[q] = (vb[q >> 5] >> (q & 31)) & 1u ? v[q] : -INFINITY;
-            mx4[q & 3] = fmaxf(mx4[q & 3], v[q]);
-          }
         } else {
 #pragma unroll
           for (int q = 0; q < HK; ++q) {
@@ -535,7 +488,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_tc_kernel(PfArgs a
       mbar_arrive(&o_free);  // the next tile's first P V may overwrite O
       if (valid) {
         uint4* dst = reinterpret_cast<uint4*>(
-            a.out + (((size_t)T.b * a.Lq + t) * a.Hq + T.hkv * G + hd) * D + hf * HD);
+            a.out + (((size_t)T.b * a.Lq + t) * a.Hq + T.hkv * G + r % G) * D + hf * HD);
 #pragma unroll
         for (int c = 0; c < HD / 8; ++c)
           dst[c] = make_uint4(pack_bf16x2(o[8 * c] * inv, o[8 * c + 1] * inv),
@@ -562,18 +515,17 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_attn_tc_kernel(PfArgs a
   }
 }
 
-template <int D, bool WIN = false>
+template <int D>
 cudaError_t launch_pf(const PfArgs& a, cudaStream_t st) {
-  auto k = prefill_attn_tc_kernel<D, WIN>;
+  auto k = prefill_attn_tc_kernel<D>;
   static PerDeviceOnce attr;
   const cudaError_t e =
       attr.run([&] { return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pf_smem(D)); });
   if (e != cudaSuccess) return e;
   // persistent: one CTA per SM (shared memory and TMEM allow one), each taking the next tile
   // left (the longest causal ranges first)
-  const int G = a.Hq / a.Hkv, TQ = kPfRows / G;
-  const long long nqt = WIN ? ((long long)a.Lq * G + kPfRows - 1) / kPfRows : (a.Lq + TQ - 1) / TQ;
-  const long long ntiles = nqt * a.B * a.Hkv;
+  const int TQ = kPfRows / (a.Hq / a.Hkv);
+  const long long ntiles = (long long)((a.Lq + TQ - 1) / TQ) * a.B * a.Hkv;
   const int grid = (int)std::min<long long>(ntiles, sm_count());
   return launch_pdl(k, dim3(grid), dim3(kPfThreads), pf_smem(D), st, a);
 }
@@ -595,11 +547,10 @@ bool prefill_attn_tc_fits(int Lq, int Hq, int Hkv, int D, const void* q, const v
          page_stride % 8 == 0 && head_stride % 8 == 0;
 }
 
-// window > 0: the kernel with a sliding window and sinks (any G)
 cudaError_t launch_prefill_attn_tc(const void* q, int B, int Lq, int Hq, int Hkv, int D, const void* kc,
                                    const void* vc, int64_t page_stride, int64_t head_stride, const int32_t* bt,
                                    int max_blocks, const int32_t* seq_lens, float scale, void* out, int* counters,
-                                   int* err, cudaStream_t st, int window, int sinks) {
+                                   int* err, cudaStream_t st) {
   PfArgs a;
   a.q = (const uint16_t*)q;
   a.kc = (const uint16_t*)kc;
@@ -617,11 +568,6 @@ cudaError_t launch_prefill_attn_tc(const void* q, int B, int Lq, int Hq, int Hkv
   a.out = (uint16_t*)out;
   a.err = err;
   a.counters = counters;
-  if (window > 0) {
-    a.window = window;
-    a.sinks = sinks;
-    return D == 64 ? launch_pf<64, true>(a, st) : launch_pf<128, true>(a, st);
-  }
   return D == 64 ? launch_pf<64>(a, st) : launch_pf<128>(a, st);
 }
 

@@ -419,8 +419,8 @@ bool window_shape_ok(int B, int Lq, int Hq, int Hkv, int D, int max_seq_len, int
          B <= 65535;
 }
 
-// Above 64 query rows per kv head the 128-row tiles of the tcgen05 kernel (prefill_attn.cu) take
-// over, as they do for higgs_paged_attention.
+// Above 64 query rows per kv head the tcgen05 kernel (window_prefill.cu) takes over, as one does for
+// higgs_paged_attention.
 bool window_on_tc(int Lq, int Hq, int Hkv) { return prefill_attn_tc_on() && (int64_t)(Hq / Hkv) * Lq > 64; }
 
 }  // namespace
@@ -469,9 +469,9 @@ extern "C" int higgs_window_attention(higgs_ctx* ctx, const void* q, int B, int 
                 "higgs_window_attention: workspace too small (need " + std::to_string(need) + " bytes)");
   HG_DEVICE(ctx);
   if (tc) {
-    HG_CUDA(launch_prefill_attn_tc(q, B, Lq, Hq, Hkv, D, k_cache, v_cache, page_stride, head_stride, block_table,
-                                   max_blocks, seq_lens, scale, out, (int*)workspace, tc_err_ptr(),
-                                   (cudaStream_t)stream, window, sinks));
+    HG_CUDA(launch_window_prefill(q, B, Lq, Hq, Hkv, D, k_cache, v_cache, page_stride, head_stride, block_table,
+                                  max_blocks, seq_lens, window, sinks, scale, out, (int*)workspace, tc_err_ptr(),
+                                  (cudaStream_t)stream));
     return HIGGS_OK;
   }
   WinArgs a;
