@@ -10,8 +10,11 @@
 //   0, 1  softmax, a thread per query row of a half: S_j from tensor memory into registers, mask,
 //         maximum and sum, P_j as bf16 over S_j's columns, and O rescaled there when a row's
 //         maximum grew by more than 2^8; at the end O / l as bf16 to memory
-//   2     loads Q and, alternating, K_j and V_j: 16-byte cp.async through the block table into
-//         128-byte-swizzled tiles of a ring (hidden keys as zeros: 0 x NaN would be NaN)
+//   2     loads Q and, alternating, K_j and V_j into 128-byte-swizzled tiles of a ring: by TMA, a box
+//         per page, or where a block has keys that no row sees (and whose slots may hold anything:
+//         0 x NaN would be NaN) by 16-byte cp.async with zeros for those.  (With cp.async for every
+//         block the loaders were the bound: each hand-over's proxy fence waits for the copies in
+//         flight, 2800 cycles a tile.)
 //   3     one warp per half issues S_j = Q K_j^T, waits for P_j, issues O += P_j V_j
 // Two halves share every K and V tile, and one half's products run while the other's softmax does:
 // S, P and O of both fill the 512 columns of tensor memory, S_j+1 waits for P_j V_j.
@@ -114,8 +117,49 @@ __device__ __forceinline__ uint32_t pack_p(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// One lane of the warp, the same each time.
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t pred;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(pred));
+  return pred;
+}
+
+// tcgen05 instructions of the elected lane in code that the whole warp runs: operands that are the
+// same for all lanes then sit in uniform registers, which these instructions take, and each costs
+// an issue slot; under a branch of one lane they are moved there first, operand by operand.
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accum) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accum), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accum) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accum), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void commit_if(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(lead)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, int d, int head, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(map), "r"(d), "r"(0), "r"(head), "r"(page), "r"(smem_u32(bar))
+      : "memory");
+}
+
 template <int D>
-__global__ void __launch_bounds__(kWpThreads, 1) window_prefill_kernel(WpArgs a) {
+__global__ void __launch_bounds__(kWpThreads, 1)
+    window_prefill_kernel(WpArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   constexpr int SLOTS = wp_slots(D), DC = D / 8;  // DC: 16-byte chunks of a row
   constexpr uint32_t kTile = wp_tile_bytes(D);
   constexpr int COL_O = 2 * kKeys;  // S (and P over it) of half x at 128 x, O at 256 + 128 x
@@ -126,6 +170,7 @@ __global__ void __launch_bounds__(kWpThreads, 1) window_prefill_kernel(WpArgs a)
   __shared__ __align__(8) uint64_t q_full, q_empty;                     // a phase per tile
   __shared__ __align__(8) uint64_t kv_full[SLOTS], kv_empty[SLOTS];
   __shared__ __align__(8) uint64_t s_full[2], p_full[2], pv_done[2];    // a phase per block
+  __shared__ __align__(8) uint64_t turn[2];                             // a phase per block: half x may take exponentials
   __shared__ __align__(8) uint64_t o_free[2];                           // a phase per tile
   __shared__ __align__(8) uint64_t t_full[kTileRing], t_empty[kTileRing];
   __shared__ int tile_ring[kTileRing];
@@ -136,10 +181,10 @@ __global__ void __launch_bounds__(kWpThreads, 1) window_prefill_kernel(WpArgs a)
   volatile int* abort = &abort_flag;
 
   if (threadIdx.x == 0) {
-    mbar_init(&q_full, 128);
+    mbar_init(&q_full, 4);
     mbar_init(&q_empty, 2);
     for (int s = 0; s < SLOTS; ++s) {
-      mbar_init(&kv_full[s], 128);
+      mbar_init(&kv_full[s], 4);
       mbar_init(&kv_empty[s], 2);
     }
     for (int x = 0; x < 2; ++x) {
@@ -147,6 +192,7 @@ __global__ void __launch_bounds__(kWpThreads, 1) window_prefill_kernel(WpArgs a)
       mbar_init(&p_full[x], 128);
       mbar_init(&pv_done[x], 1);
       mbar_init(&o_free[x], 128);
+      mbar_init(&turn[x], 4);
     }
     for (int i = 0; i < kTileRing; ++i) {
       mbar_init(&t_full[i], 1);
@@ -185,10 +231,14 @@ __global__ void __launch_bounds__(kWpThreads, 1) window_prefill_kernel(WpArgs a)
     static_assert(KSTEP % 8 == 0, "a thread's rows share their swizzle");
     const uint32_t so = (dc >> 3) * (kKeys * 128) + k0 * 128 + (((dc & 7) ^ (k0 & 7)) << 4);
     const uint32_t q_addr = smem_u32(qs) + so, ring_addr = smem_u32(ring) + so;
-    int n = 0, filled = 0;  // ring tiles issued; handed over
-    auto hand_over = [&](int upto) {  // (their copies are done)
+    int n = 0;  // ring tiles issued
+    // this warp's part of a tile is in shared memory: generic writes before the tensor core's reads
+    auto arrive_after_copies = [&](uint64_t* bar) {
+      cp_async_commit();
+      cp_async_wait<0>();
       fence_proxy_async();
-      for (; filled < upto; ++filled) mbar_arrive(&kv_full[filled % SLOTS]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
     };
     for (int k = 0;; ++k) {
       if (lt == 0) {
@@ -204,46 +254,64 @@ __global__ void __launch_bounds__(kWpThreads, 1) window_prefill_kernel(WpArgs a)
       asm volatile("bar.sync 1, 128;" ::: "memory");
       if (i >= a.tiles) break;
       const WpTile T(a, i);
-      if (k >= 1) wp_wait(&q_empty, (k - 1) & 1, abort, a.err);
-#pragma unroll 4
-      for (int r = k0; r < kTileRows; r += KSTEP) {
-        const int rr = T.r0 + r, t = rr / a.G, hd = rr - t * a.G;
-        const bool ok = rr < T.r_end;
-        const uint16_t* src = a.q + (((size_t)T.b * a.Lq + (ok ? t : 0)) * a.Hq + T.h * a.G + hd) * D + dc * 8;
-        cp_async16_or_zero(q_addr + (r >> 7) * kTile + ((r & 127) - k0) * 128, src, ok);
-      }
-      cp_async_commit();
-      cp_async_wait<0>();
-      fence_proxy_async();
-      mbar_arrive(&q_full);
       const int32_t* bt = a.bt + (size_t)T.b * a.max_blocks;
       const size_t col = (size_t)T.h * a.head_stride + dc * 8;
-      for (int j = 0; j < T.blocks; ++j) {
-        const int kb = T.key(j);
-        int64_t off[KPT];  // < 0: a key that no row sees; its page is not looked up, it may be free
+      for (int j = 0; j < max(1, T.blocks); ++j) {
+        if (j < T.blocks) {
+          const int kb = T.key(j);
+          // a block all of whose keys are seen by some row comes by TMA, a box per page and 64 of d
+          const bool whole = T.is_sink(j) ? kb + kKeys <= T.sink_keys
+                                          : kb + kKeys <= T.kv_len && (kb >= T.lo || kb + kKeys <= a.sinks);
+          if (whole) {
+            const int box = lane % (8 * (D / 64)), page = bt[(kb >> 4) + box / (D / 64)], panel = box % (D / 64);
 #pragma unroll
-        for (int q = 0; q < KPT; ++q) {
-          const int kg = kb + k0 + q * KSTEP;
-          const bool ok = T.is_sink(j) ? kg < T.sink_keys : kg < T.kv_len && (kg >= T.lo || kg < a.sinks);
-          off[q] = ok ? (int64_t)bt[kg >> 4] * a.page_stride + (int64_t)col + (kg & 15) * D : -1;
-        }
+            for (int v = 0; v < 2; ++v, ++n) {
+              const int s = n % SLOTS;
+              if (n >= SLOTS) wp_wait(&kv_empty[s], ((n / SLOTS) - 1) & 1, abort, a.err);
+              __syncwarp();
+              if (lane == 0) {
+                if (warp == 8)
+                  mbar_arrive_expect_tx(&kv_full[s], kTile);
+                else
+                  mbar_arrive(&kv_full[s]);
+              }
+              __syncwarp();
+              if (warp == 8 && lane < 8 * (D / 64))
+                tma_page(smem_u32(ring) + s * kTile + panel * (kKeys * 128) + (box / (D / 64)) * 2048,
+                         v ? &v_map : &k_map, panel * 64, T.h, page, &kv_full[s]);
+            }
+          } else {
+            int64_t off[KPT];  // < 0: a key that no row sees; its page is not looked up, it may be free
 #pragma unroll
-        for (int v = 0; v < 2; ++v, ++n) {
-          const int s = n % SLOTS;
-          if (n >= SLOTS) wp_wait(&kv_empty[s], ((n / SLOTS) - 1) & 1, abort, a.err);
-          const uint16_t* pool = v ? a.vc : a.kc;
+            for (int q = 0; q < KPT; ++q) {
+              const int kg = kb + k0 + q * KSTEP;
+              const bool ok = T.is_sink(j) ? kg < T.sink_keys : kg < T.kv_len && (kg >= T.lo || kg < a.sinks);
+              off[q] = ok ? (int64_t)bt[kg >> 4] * a.page_stride + (int64_t)col + (kg & 15) * D : -1;
+            }
 #pragma unroll
-          for (int q = 0; q < KPT; ++q)
-            cp_async16_or_zero(ring_addr + s * kTile + q * KSTEP * 128, pool + (off[q] < 0 ? 0 : off[q]), off[q] >= 0);
-          cp_async_commit();
-          if (n - filled >= 2) {
-            cp_async_wait<2>();
-            hand_over(n - 1);
+            for (int v = 0; v < 2; ++v, ++n) {
+              const int s = n % SLOTS;
+              if (n >= SLOTS) wp_wait(&kv_empty[s], ((n / SLOTS) - 1) & 1, abort, a.err);
+              const uint16_t* pool = v ? a.vc : a.kc;
+#pragma unroll
+              for (int q = 0; q < KPT; ++q)
+                cp_async16_or_zero(ring_addr + s * kTile + q * KSTEP * 128, pool + (off[q] < 0 ? 0 : off[q]), off[q] >= 0);
+              arrive_after_copies(&kv_full[s]);
+            }
           }
         }
+        if (j > 0) continue;
+        // Q, once the tile before has had its last scores (the first K and V are on their way)
+        if (k >= 1) wp_wait(&q_empty, (k - 1) & 1, abort, a.err);
+#pragma unroll 4
+        for (int r = k0; r < kTileRows; r += KSTEP) {
+          const int rr = T.r0 + r, t = rr / a.G, hd = rr - t * a.G;
+          const bool ok = rr < T.r_end;
+          const uint16_t* src = a.q + (((size_t)T.b * a.Lq + (ok ? t : 0)) * a.Hq + T.h * a.G + hd) * D + dc * 8;
+          cp_async16_or_zero(q_addr + (r >> 7) * kTile + ((r & 127) - k0) * 128, src, ok);
+        }
+        arrive_after_copies(&q_full);
       }
-      cp_async_wait<0>();
-      hand_over(n);
     }
   } else if (group == 3) {
     // ---------------- MMA issue: warp 12 + x for half x ----------------
@@ -252,10 +320,11 @@ __global__ void __launch_bounds__(kWpThreads, 1) window_prefill_kernel(WpArgs a)
     if (x < 2) {
       constexpr uint32_t idS = tc_idesc_bf16(kM, kKeys), idO = tc_idesc_bf16(kM, D, true);
       const uint32_t sq = smem_u32(qs) + x * kTile, sr = smem_u32(ring);
-      const uint32_t col_s = tb + x * kKeys, col_o = tb + COL_O + x * kKeys;
+      const uint32_t ub = __shfl_sync(0xffffffffu, tb, 0);
+      const uint32_t col_s = ub + x * kKeys, col_o = ub + COL_O + x * kKeys, lead = elect_lane();
       int J = 0;
       for (int k = 0;; ++k) {
-        const int i = next_tile(k, lane == 0);
+        const int i = next_tile(k, lead != 0);
         if (i >= a.tiles) break;
         const WpTile T(a, i);
         wp_wait(&q_full, k & 1, abort, a.err);
@@ -263,35 +332,28 @@ __global__ void __launch_bounds__(kWpThreads, 1) window_prefill_kernel(WpArgs a)
           const int ks = (2 * J) % SLOTS, vs = (2 * J + 1) % SLOTS;
           wp_wait(&kv_full[ks], ((2 * J) / SLOTS) & 1, abort, a.err);
           tc_fence_after();
-          if (lane == 0) {
-            const uint32_t sk = sr + ks * kTile;
+          const uint32_t sk = sr + ks * kTile;
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-              tc_mma(col_s, sw128_desc(sq + (kk >> 2) * (kM * 128) + (kk & 3) * 32),
-                     sw128_desc(sk + (kk >> 2) * (kKeys * 128) + (kk & 3) * 32), idS, kk > 0 ? 1u : 0u);
-            tc_commit(&s_full[x]);
-            tc_commit(&kv_empty[ks]);
-            if (j == T.blocks - 1) tc_commit(&q_empty);
-          }
-          __syncwarp();
+          for (int kk = 0; kk < D / 16; ++kk)
+            mma_ss(lead, col_s, sw128_desc(sq + (kk >> 2) * (kM * 128) + (kk & 3) * 32),
+                   sw128_desc(sk + (kk >> 2) * (kKeys * 128) + (kk & 3) * 32), idS, kk > 0);
+          commit_if(lead, &s_full[x]);
+          commit_if(lead, &kv_empty[ks]);
+          if (j == T.blocks - 1) commit_if(lead, &q_empty);
           wp_wait(&kv_full[vs], ((2 * J + 1) / SLOTS) & 1, abort, a.err);
           // a tile's first product overwrites O: its threads have read the tile's before
           if (j == 0 && k >= 1) wp_wait(&o_free[x], (k - 1) & 1, abort, a.err);
           wp_wait(&p_full[x], J & 1, abort, a.err);
           tc_fence_after();
-          if (lane == 0) {
-            const uint32_t sv = sr + vs * kTile;
+          const uint32_t sv = sr + vs * kTile;
 #pragma unroll
-            for (int kk = 0; kk < kKeys / 16; ++kk)  // 16 keys = two 8-row atoms = 2 KB
-              tc_mma_ta(col_o, col_s + kk * 8, sw128_mn_desc(sv + kk * 2048, kKeys * 128), idO,
-                        (j > 0 || kk > 0) ? 1u : 0u);
-            tc_commit(&pv_done[x]);
-            tc_commit(&kv_empty[vs]);
-          }
-          __syncwarp();
+          for (int kk = 0; kk < kKeys / 16; ++kk)  // 16 keys = two 8-row atoms = 2 KB
+            mma_ts(lead, col_o, col_s + kk * 8, sw128_mn_desc(sv + kk * 2048, kKeys * 128), idO, j > 0 || kk > 0);
+          commit_if(lead, &pv_done[x]);
+          commit_if(lead, &kv_empty[vs]);
           wp_wait(&pv_done[x], J & 1, abort, a.err);  // the next S overwrites P
         }
-        if (T.blocks == 0 && lane == 0) mbar_arrive(&q_empty);
+        if (T.blocks == 0 && lead) mbar_arrive(&q_empty);
       }
     }
   } else {
@@ -334,7 +396,9 @@ __global__ void __launch_bounds__(kWpThreads, 1) window_prefill_kernel(WpArgs a)
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int q = 0; q < kKeys; ++q) mx4[q & 3] = fmaxf(mx4[q & 3], v[q]);
+        for (int q = 0; q < kKeys; q += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx4[e] = fmaxf(mx4[e], fmaxf(v[q + e], v[q + 4 + e]));
         // raw scores: the scale (> 0) is applied to the maximum and folded into the exponent's FMA
         const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
         const bool grow = mx > m + kWpSlack || (m == -INFINITY && mx != -INFINITY);
@@ -356,6 +420,12 @@ __global__ void __launch_bounds__(kWpThreads, 1) window_prefill_kernel(WpArgs a)
             }
           }
         }
+        // The halves take their exponentials in turn: each then has the special-function units to
+        // itself while the other's products run, instead of both waiting for the one, then the other.
+        if (x == 1)
+          wp_wait(&turn[1], J & 1, abort, a.err);
+        else if (J > 0)
+          wp_wait(&turn[0], (J - 1) & 1, abort, a.err);
         const float mm = m == -INFINITY ? 0.f : m;  // (nothing visible yet: every score is -inf)
         const float2 neg_m = make_float2(-mm, -mm);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -371,6 +441,8 @@ __global__ void __launch_bounds__(kWpThreads, 1) window_prefill_kernel(WpArgs a)
           }
           tc_st16(col_s + 16 * c, pk);
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&turn[x ^ 1]);
         l2 = __fadd2_rn(l2, __fadd2_rn(sum[0], sum[1]));
         tc_wait_st();
         tc_fence_before();
@@ -423,14 +495,45 @@ __global__ void __launch_bounds__(kWpThreads, 1) window_prefill_kernel(WpArgs a)
   }
 }
 
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// A pool as [pages, kv heads, 16, D], in boxes of one head's page by 64 of d, 128-byte swizzle.
+bool pool_map(const void* pool, int Hkv, int D, int64_t page_stride, int64_t head_stride, CUtensorMap* out) {
+  static EncodeFn encode = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                   q == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<EncodeFn>(p)
+               : nullptr;
+  }();
+  if (!encode) return false;
+  // (the number of pages is not known here: ids come from the block table; the stride of a
+  // dimension of one head is never used)
+  const cuuint64_t dims[4] = {(cuuint64_t)D, HIGGS_PAGE_SIZE, (cuuint64_t)Hkv, (cuuint64_t)INT32_MAX};
+  const cuuint64_t strides[3] = {(cuuint64_t)D * 2,
+                                 Hkv == 1 ? (cuuint64_t)D * 2 * HIGGS_PAGE_SIZE : (cuuint64_t)head_stride * 2,
+                                 (cuuint64_t)page_stride * 2};
+  const cuuint32_t box[4] = {64, HIGGS_PAGE_SIZE, 1, 1}, step[4] = {1, 1, 1, 1};
+  return encode(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(pool), dims, strides, box, step,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D>
 cudaError_t launch_wp(const WpArgs& a, cudaStream_t st) {
+  CUtensorMap k_map, v_map;
+  if (!pool_map(a.kc, a.Hkv, D, a.page_stride, a.head_stride, &k_map) ||
+      !pool_map(a.vc, a.Hkv, D, a.page_stride, a.head_stride, &v_map))
+    return cudaErrorInvalidValue;
   auto k = window_prefill_kernel<D>;
   static PerDeviceOnce attr;
   const cudaError_t e =
       attr.run([&] { return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)wp_smem(D)); });
   if (e != cudaSuccess) return e;
-  return launch_pdl(k, dim3(std::min(a.tiles, sm_count())), dim3(kWpThreads), wp_smem(D), st, a);
+  return launch_pdl(k, dim3(std::min(a.tiles, sm_count())), dim3(kWpThreads), wp_smem(D), st, a, k_map, v_map);
 }
 
 }  // namespace
