@@ -7,18 +7,16 @@
 // that some row of it sees in blocks of 128: blocks from key 0 for the sinks, then from the page
 // where the window of its first token starts.  The kernel is persistent, a CTA per SM taking the
 // next tile from a counter, with the rings running on from tile to tile.  The warpgroups:
-//   0, 1  softmax, a thread per query row of a half: S_j from tensor memory into registers, mask,
-//         maximum and sum, P_j as bf16 over S_j's columns, and O rescaled there when a row's
-//         maximum grew by more than 2^8; at the end O / l as bf16 to memory
-//   2     loads Q and, alternating, K_j and V_j into 128-byte-swizzled tiles of a ring: by TMA, a box
-//         per page, or where a block has keys that no row sees (and whose slots may hold anything:
-//         0 x NaN would be NaN) by 16-byte cp.async with zeros for those.  (With cp.async for every
-//         block the loaders were the bound: each hand-over's proxy fence waits for the copies in
-//         flight, 2800 cycles a tile.)
-//   3     one warp per half issues S_j = Q K_j^T, waits for P_j, issues O += P_j V_j
-// Two halves share every K and V tile, and one half's products run while the other's softmax does:
-// S, P and O of both fill the 512 columns of tensor memory, S_j+1 waits for P_j V_j.
-// Registers: 192 for softmax threads (a row's 128 scores stay in them), 64 for the others.
+//   0, 1  softmax, a thread per query row of a half, 64 keys at a time: S_u from tensor memory into
+//         registers, mask, maximum and sum, P_u as bf16 over S_u's columns, and O rescaled there
+//         when a row's maximum grew by more than 2^8; at the end O / l as bf16 to memory
+//   2     loads Q and, alternating, K_j and V_j of 128 keys into 128-byte-swizzled tiles of a ring: by
+//         TMA, a box per page, or where a block has keys that no row sees (and whose slots may hold
+//         anything: 0 x NaN would be NaN) by 16-byte cp.async with zeros for those
+//   3     one warp per half issues S_u = Q K_u^T two steps ahead, waits for P_u, issues O += P_u V_u
+// S, P and O of both halves fill the 512 columns of tensor memory: per half two buffers of 64 scores
+// and 128 of O.  S_u+1 waits there while the softmax of S_u runs, S_u+2 is issued when P_u V_u is done.
+// Both halves share every K and V tile.
 // Every mbarrier wait is bounded (about 2 s; the first timeout makes the CTA's other waits give up
 // and sets the flag that higgs_tc_error reports).
 #include <algorithm>
@@ -32,7 +30,8 @@ namespace {
 
 constexpr int kM = 128;          // rows of a half (UMMA M)
 constexpr int kTileRows = 2 * kM;
-constexpr int kKeys = 128;       // keys of a block
+constexpr int kKeys = 128;       // keys of a block, loaded as one tile of K and one of V
+constexpr int kHalf = 64;        // keys of half a block: the scores' and weights' unit
 constexpr int kWpThreads = 512;  // warpgroups: softmax x 2, loaders, MMA issue
 constexpr int kWpTmemCols = 512;
 constexpr int kTileRing = 4;     // tile indices handed from the first loader thread to the others
@@ -162,15 +161,14 @@ __global__ void __launch_bounds__(kWpThreads, 1)
     window_prefill_kernel(WpArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   constexpr int SLOTS = wp_slots(D), DC = D / 8;  // DC: 16-byte chunks of a row
   constexpr uint32_t kTile = wp_tile_bytes(D);
-  constexpr int COL_O = 2 * kKeys;  // S (and P over it) of half x at 128 x, O at 256 + 128 x
+  constexpr int COL_O = 2 * kM;  // S (and P over it) of half x, buffer u & 1, at 128 x + 64 (u & 1); O at 256 + 128 x
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* qs = smem;               // [half][D / 64 panels][128 rows][128 B], 128-byte swizzle
   uint8_t* ring = smem + 2 * kTile;  // K_0, V_0, K_1, ... of all the CTA's tiles: [D / 64][128 keys][128 B]
   __shared__ __align__(8) uint64_t q_full, q_empty;                     // a phase per tile
   __shared__ __align__(8) uint64_t kv_full[SLOTS], kv_empty[SLOTS];
-  __shared__ __align__(8) uint64_t s_full[2], p_full[2], pv_done[2];    // a phase per block
-  __shared__ __align__(8) uint64_t turn[2];                             // a phase per block: half x may take exponentials
+  __shared__ __align__(8) uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];  // [half][buffer]
   __shared__ __align__(8) uint64_t o_free[2];                           // a phase per tile
   __shared__ __align__(8) uint64_t t_full[kTileRing], t_empty[kTileRing];
   __shared__ int tile_ring[kTileRing];
@@ -188,11 +186,12 @@ __global__ void __launch_bounds__(kWpThreads, 1)
       mbar_init(&kv_empty[s], 2);
     }
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[x], 128);
-      mbar_init(&pv_done[x], 1);
+      for (int u = 0; u < 2; ++u) {
+        mbar_init(&s_full[x][u], 1);
+        mbar_init(&p_full[x][u], 128);
+        mbar_init(&pv_done[x][u], 1);
+      }
       mbar_init(&o_free[x], 128);
-      mbar_init(&turn[x], 4);
     }
     for (int i = 0; i < kTileRing; ++i) {
       mbar_init(&t_full[i], 1);
@@ -224,7 +223,6 @@ __global__ void __launch_bounds__(kWpThreads, 1)
 
   if (group == 2) {
     // ---------------- loaders ----------------
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     const int lt = threadIdx.x - 256;
     constexpr int KSTEP = 128 / DC, KPT = kKeys / KSTEP;  // rows of a tile per thread, KSTEP apart
     const int dc = lt % DC, k0 = lt / DC;
@@ -315,55 +313,64 @@ __global__ void __launch_bounds__(kWpThreads, 1)
     }
   } else if (group == 3) {
     // ---------------- MMA issue: warp 12 + x for half x ----------------
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     const int x = warp - 12;
     if (x < 2) {
-      constexpr uint32_t idS = tc_idesc_bf16(kM, kKeys), idO = tc_idesc_bf16(kM, D, true);
-      const uint32_t sq = smem_u32(qs) + x * kTile, sr = smem_u32(ring);
+      constexpr uint32_t idS = tc_idesc_bf16(kM, kHalf), idO = tc_idesc_bf16(kM, D, true);
+      const uint32_t sq = smem_u32(qs) + x * kTile, sr = smem_u32(ring), lead = elect_lane();
       const uint32_t ub = __shfl_sync(0xffffffffu, tb, 0);
-      const uint32_t col_s = ub + x * kKeys, col_o = ub + COL_O + x * kKeys, lead = elect_lane();
-      int J = 0;
+      const uint32_t col_s = ub + x * kM, col_o = ub + COL_O + x * kM;
+      int U = 0;  // half blocks of the CTA's tiles before this one; K of half block u is ring tile u & ~1, V the next
       for (int k = 0;; ++k) {
         const int i = next_tile(k, lead != 0);
         if (i >= a.tiles) break;
         const WpTile T(a, i);
+        const int n = 2 * T.blocks;
         wp_wait(&q_full, k & 1, abort, a.err);
-        for (int j = 0; j < T.blocks; ++j, ++J) {
-          const int ks = (2 * J) % SLOTS, vs = (2 * J + 1) % SLOTS;
-          wp_wait(&kv_full[ks], ((2 * J) / SLOTS) & 1, abort, a.err);
+        auto scores = [&](int u) {  // S_u = Q K_u^T, into the buffer that P_{u-2} V_{u-2} has read
+          const int g = U + u, slot = (g & ~1) % SLOTS;
+          if (!(u & 1)) wp_wait(&kv_full[slot], ((g & ~1) / SLOTS) & 1, abort, a.err);
           tc_fence_after();
-          const uint32_t sk = sr + ks * kTile;
+          const uint32_t sk = sr + slot * kTile + (u & 1) * (kHalf * 128), cs = col_s + (u & 1) * kHalf;
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
-            mma_ss(lead, col_s, sw128_desc(sq + (kk >> 2) * (kM * 128) + (kk & 3) * 32),
+            mma_ss(lead, cs, sw128_desc(sq + (kk >> 2) * (kM * 128) + (kk & 3) * 32),
                    sw128_desc(sk + (kk >> 2) * (kKeys * 128) + (kk & 3) * 32), idS, kk > 0);
-          commit_if(lead, &s_full[x]);
-          commit_if(lead, &kv_empty[ks]);
-          if (j == T.blocks - 1) commit_if(lead, &q_empty);
-          wp_wait(&kv_full[vs], ((2 * J + 1) / SLOTS) & 1, abort, a.err);
-          // a tile's first product overwrites O: its threads have read the tile's before
-          if (j == 0 && k >= 1) wp_wait(&o_free[x], (k - 1) & 1, abort, a.err);
-          wp_wait(&p_full[x], J & 1, abort, a.err);
-          tc_fence_after();
-          const uint32_t sv = sr + vs * kTile;
-#pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk)  // 16 keys = two 8-row atoms = 2 KB
-            mma_ts(lead, col_o, col_s + kk * 8, sw128_mn_desc(sv + kk * 2048, kKeys * 128), idO, j > 0 || kk > 0);
-          commit_if(lead, &pv_done[x]);
-          commit_if(lead, &kv_empty[vs]);
-          wp_wait(&pv_done[x], J & 1, abort, a.err);  // the next S overwrites P
+          commit_if(lead, &s_full[x][u & 1]);
+          if (u & 1) commit_if(lead, &kv_empty[slot]);
+          if (u == n - 1) commit_if(lead, &q_empty);
+        };
+        if (n > 0) {
+          scores(0);
+          scores(1);
+        } else if (lead) {
+          mbar_arrive(&q_empty);
         }
-        if (T.blocks == 0 && lead) mbar_arrive(&q_empty);
+        for (int u = 0; u < n; ++u) {
+          const int g = U + u, slot = (g | 1) % SLOTS, phase = (g >> 1) & 1;
+          if (!(u & 1)) wp_wait(&kv_full[slot], ((g | 1) / SLOTS) & 1, abort, a.err);
+          // a tile's first product overwrites O: its threads have read the tile's before
+          if (u == 0 && k >= 1) wp_wait(&o_free[x], (k - 1) & 1, abort, a.err);
+          wp_wait(&p_full[x][u & 1], phase, abort, a.err);
+          tc_fence_after();
+          const uint32_t sv = sr + slot * kTile + (u & 1) * (kHalf * 128), cs = col_s + (u & 1) * kHalf;
+#pragma unroll
+          for (int kk = 0; kk < kHalf / 16; ++kk)  // 16 keys = two 8-row atoms = 2 KB
+            mma_ts(lead, col_o, cs + kk * 8, sw128_mn_desc(sv + kk * 2048, kKeys * 128), idO, u > 0 || kk > 0);
+          commit_if(lead, &pv_done[x][u & 1]);
+          if (u & 1) commit_if(lead, &kv_empty[slot]);
+          wp_wait(&pv_done[x][u & 1], phase, abort, a.err);  // (what is next overwrites P)
+          if (u + 2 < n) scores(u + 2);
+        }
+        U += n;
       }
     }
   } else {
     // ---------------- softmax: half x, a thread per row ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     const int x = group, r = x * kM + (threadIdx.x & 127);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t col_s = tb + lanes + x * kKeys, col_o = tb + lanes + COL_O + x * kKeys;
+    const uint32_t col_s = tb + lanes + x * kM, col_o = tb + lanes + COL_O + x * kM;
     const float2 scale2 = make_float2(a.scale_log2, a.scale_log2);
-    int J = 0;
+    int U = 0;
     for (int k = 0;; ++k) {
       const int i = next_tile(k, true);
       if (i >= a.tiles) break;
@@ -373,22 +380,26 @@ __global__ void __launch_bounds__(kWpThreads, 1)
       const int pos = valid ? T.first + t : -1;
       float m = -INFINITY;
       float2 l2 = make_float2(0.f, 0.f);
-      for (int j = 0; j < T.blocks; ++j, ++J) {
-        wp_wait(&s_full[x], J & 1, abort, a.err);
+      const int n = 2 * T.blocks;
+      for (int u = 0; u < n; ++u) {
+        const int buf = u & 1, phase = ((U + u) >> 1) & 1;
+        const uint32_t cs = col_s + buf * kHalf;
+        wp_wait(&s_full[x][buf], phase, abort, a.err);
         tc_fence_after();
-        float v[kKeys];
+        float v[kHalf];
 #pragma unroll
-        for (int c = 0; c < kKeys / 16; ++c) tc_ld16(col_s + 16 * c, v + 16 * c);
-        tc_wait_ld();
-        // key i of the block is visible iff i <= lim and (i >= low or i < snk)
-        const int kb = T.key(j);
-        int lim = pos - kb;
+        for (int c = 0; c < kHalf / 16; ++c) tc_ld16(cs + 16 * c, v + 16 * c);
+        // key i of the half block is visible iff i <= lim and (i >= low or i < snk)
+        const bool sink = T.is_sink(u >> 1);
+        const int kb = T.key(u >> 1) + buf * kHalf;
+        const int lim = sink ? min(pos, T.sink_keys - 1) - kb : pos - kb;
         const int low = pos - a.window + 1 - kb, snk = a.sinks - kb;
-        if (T.is_sink(j)) lim = min(lim, T.sink_keys - 1 - kb);
-        if (!__all_sync(0xffffffffu, lim >= kKeys - 1 && (low <= 0 || snk >= kKeys))) {
+        const bool whole = __all_sync(0xffffffffu, lim >= kHalf - 1 && (low <= 0 || snk >= kHalf));
+        tc_wait_ld();
+        if (!whole) {
           auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
 #pragma unroll
-          for (int c = 0; c < kKeys / 32; ++c) {
+          for (int c = 0; c < kHalf / 32; ++c) {
             const uint32_t vis = below(lim + 1 - 32 * c) & (~below(low - 32 * c) | below(snk - 32 * c));
 #pragma unroll
             for (int q = 0; q < 32; ++q) v[32 * c + q] = (vis >> q) & 1u ? v[32 * c + q] : -INFINITY;
@@ -396,7 +407,7 @@ __global__ void __launch_bounds__(kWpThreads, 1)
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int q = 0; q < kKeys; q += 8)
+        for (int q = 0; q < kHalf; q += 8)
 #pragma unroll
           for (int e = 0; e < 4; ++e) mx4[e] = fmaxf(mx4[e], fmaxf(v[q + e], v[q + 4 + e]));
         // raw scores: the scale (> 0) is applied to the maximum and folded into the exponent's FMA
@@ -407,7 +418,9 @@ __global__ void __launch_bounds__(kWpThreads, 1)
           if (grow) m = mx;
           l2.x *= alpha;
           l2.y *= alpha;
-          if (j >= 1) {  // S_j was issued after P_{j-1} V_{j-1} had completed
+          if (u >= 1) {
+            wp_wait(&pv_done[x][buf ^ 1], ((U + u - 1) >> 1) & 1, abort, a.err);
+            tc_fence_after();
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
               float o[16];
@@ -420,17 +433,11 @@ __global__ void __launch_bounds__(kWpThreads, 1)
             }
           }
         }
-        // The halves take their exponentials in turn: each then has the special-function units to
-        // itself while the other's products run, instead of both waiting for the one, then the other.
-        if (x == 1)
-          wp_wait(&turn[1], J & 1, abort, a.err);
-        else if (J > 0)
-          wp_wait(&turn[0], (J - 1) & 1, abort, a.err);
         const float mm = m == -INFINITY ? 0.f : m;  // (nothing visible yet: every score is -inf)
         const float2 neg_m = make_float2(-mm, -mm);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int c = 0; c < kKeys / 32; ++c) {
+        for (int c = 0; c < kHalf / 32; ++c) {
           uint32_t pk[16];
 #pragma unroll
           for (int q = 0; q < 16; ++q) {
@@ -439,18 +446,17 @@ __global__ void __launch_bounds__(kWpThreads, 1)
             sum[q & 1] = __fadd2_rn(sum[q & 1], p);
             pk[q] = pack_p(p.x, p.y);
           }
-          tc_st16(col_s + 16 * c, pk);
+          tc_st16(cs + 16 * c, pk);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&turn[x ^ 1]);
         l2 = __fadd2_rn(l2, __fadd2_rn(sum[0], sum[1]));
         tc_wait_st();
         tc_fence_before();
-        mbar_arrive(&p_full[x]);
+        mbar_arrive(&p_full[x][buf]);
       }
+      U += n;
       // ---- O / l -> bf16 ----
       if (T.blocks > 0) {
-        wp_wait(&pv_done[x], (J - 1) & 1, abort, a.err);
+        wp_wait(&pv_done[x][1], ((U - 1) >> 1) & 1, abort, a.err);
         tc_fence_after();
       }
       const float l = l2.x + l2.y, inv = l > 0.f ? 1.f / l : 0.f;
