@@ -135,12 +135,11 @@ extern "C" int higgs_kv_copy_pages(higgs_ctx* ctx, const higgs_kv_pool* pools, i
   if (int rc = check_pairs(src, dst, n, pages)) return rc;
   HG_DEVICE(ctx);
   // parameters are copied at every launch, so short lists use a short argument block
-  constexpr int kSmall = 64, kLarge = 1024;
+  constexpr int kSmall = 16, kMiddle = 128, kLarge = 1024;
   for (int i = 0; i < n; i += kLarge) {
     const int m = std::min(kLarge, n - i);
-    const int rc = m <= kSmall ? launch_copy<kSmall>(pools, n_pools, src + i, dst + i, m, (cudaStream_t)stream)
-                               : launch_copy<kLarge>(pools, n_pools, src + i, dst + i, m, (cudaStream_t)stream);
-    if (rc) return rc;
+    const auto launch = m <= kSmall ? launch_copy<kSmall> : m <= kMiddle ? launch_copy<kMiddle> : launch_copy<kLarge>;
+    if (int rc = launch(pools, n_pools, src + i, dst + i, m, (cudaStream_t)stream)) return rc;
   }
   return HIGGS_OK;
 } catch (const std::bad_alloc&) {

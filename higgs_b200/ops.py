@@ -305,38 +305,41 @@ def window_attention(q, k_cache, v_cache, block_table, seq_lens, max_seq_len: in
     q bf16 [B, Lq, Hq, D], contiguous; caches bf16 [num_pages, Hkv, 16, D], of equal strides, each
     (page, head) block contiguous; block_table int32 [B, max_blocks], whose entries of pages no
     query sees may hold anything; seq_lens int32 [B], at most max_seq_len.  Returns bf16 [B, Lq, Hq, D]."""
-    _chk(q, torch.bfloat16, "q")
-    _chk(block_table, torch.int32, "block_table")
-    _chk(seq_lens, torch.int32, "seq_lens")
-    if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16:
-        raise TypeError(f"the caches must be torch.bfloat16, got {k_cache.dtype} and {v_cache.dtype}")
+    if (q.dtype is not torch.bfloat16 or k_cache.dtype is not torch.bfloat16 or
+            v_cache.dtype is not torch.bfloat16 or block_table.dtype is not torch.int32 or
+            seq_lens.dtype is not torch.int32):
+        raise TypeError("q and the caches must be torch.bfloat16, block_table and seq_lens torch.int32")
     shape, strides = k_cache.shape, k_cache.stride()
-    if q.dim() != 4 or len(shape) != 4:
-        raise ValueError("q must be [B, Lq, Hq, D] and the caches [num_pages, Hkv, 16, D]")
+    if len(q.shape) != 4 or len(shape) != 4 or len(block_table.shape) != 2:
+        raise ValueError("q must be [B, Lq, Hq, D], the caches [num_pages, Hkv, 16, D], block_table "
+                         "[B, max_blocks]")
     B, Lq, Hq, D = q.shape
+    Hkv, max_blocks = shape[1], block_table.shape[1]
     if shape[2] != PAGE or shape[3] != D or v_cache.shape != shape:
         raise ValueError(f"the caches must be [num_pages, Hkv, {PAGE}, {D}], got {list(shape)} and "
                          f"{list(v_cache.shape)}")
     if v_cache.stride() != strides or strides[2] != D or strides[3] != 1:
         raise ValueError("the caches need equal strides and contiguous (page, head) blocks")
-    if block_table.dim() != 2 or block_table.shape[0] != B or seq_lens.shape != (B,):
+    if block_table.shape[0] != B or seq_lens.shape != (B,):
         raise ValueError("block_table must be [B, max_blocks] and seq_lens [B]")
+    if not (q.is_contiguous() and block_table.is_contiguous() and seq_lens.is_contiguous()):
+        raise ValueError("q, block_table and seq_lens must be contiguous")
     ctx = _ctx(q)
     _same_device(q, k_cache, v_cache, block_table, seq_lens, workspace)
-    Hkv = shape[1]
-    if scale is None:
-        scale = 1.0 / math.sqrt(D)
     if workspace is None:
         workspace = window_attention_workspace(B, Lq, Hq, Hkv, D, max_seq_len, window, sinks, q.device)
     out = torch.empty_like(q)
     ffi.call("higgs_window_attention", ctx, q.data_ptr(), B, Lq, Hq, Hkv, D, k_cache.data_ptr(),
-             v_cache.data_ptr(), strides[0], strides[1], block_table.data_ptr(), block_table.shape[1],
-             seq_lens.data_ptr(), int(max_seq_len), int(window), int(sinks), float(scale), out.data_ptr(),
-             workspace.data_ptr(), workspace.numel(), _st(q.device))
+             v_cache.data_ptr(), strides[0], strides[1], block_table.data_ptr(), max_blocks,
+             seq_lens.data_ptr(), int(max_seq_len), int(window), int(sinks),
+             D ** -0.5 if scale is None else float(scale), out.data_ptr(), workspace.data_ptr(),
+             workspace.numel(), _st(q.device))
     return out
 
 
 def _page_list(a) -> np.ndarray:
+    if type(a) is np.ndarray and a.dtype == np.int32 and a.ndim == 1 and a.flags.c_contiguous:
+        return a
     a = np.asarray(a)
     if a.dtype != np.int32:
         if a.size and (a.dtype.kind not in "iu" or int(a.max()) > 2 ** 31 - 1 or int(a.min()) < -2 ** 31):
@@ -357,15 +360,11 @@ def kv_copy_pages(pools, src, dst) -> None:
     words = []  # higgs_kv_pool: six 8-byte fields
     for t in pools:
         shape, strides, es = t.shape, t.stride(), t.element_size()
-        page = 1
-        for n, st in zip(reversed(shape[2:]), reversed(strides[2:])):
-            if n != 1 and st != page:
-                page = -1
-                break
-            page *= n
-        if len(shape) < 3 or page < 0:
+        if len(shape) < 3 or not (t.is_contiguous() or t[:1, :1].is_contiguous()):
             raise ValueError("a pool must be [layers, num_pages, ...] with contiguous pages")
-        words += (t.data_ptr(), shape[0], shape[1], strides[0] * es, strides[1] * es, page * es)
+        layers, pages = shape[0], shape[1]
+        words += (t.data_ptr(), layers, pages, strides[0] * es, strides[1] * es,
+                  t.numel() // max(layers * pages, 1) * es)
     _same_device(*pools)
     ffi.call("higgs_kv_copy_pages", _ctx(pools[0]), (ctypes.c_int64 * len(words))(*words), len(pools),
              src.__array_interface__["data"][0], dst.__array_interface__["data"][0], src.size,
@@ -470,25 +469,26 @@ def beam_select(logits, scores, n_out: int, workspace=None):
 
     logits f32 [B * beams, V] or [B, beams, V]; scores f32 [B, beams].  Returns (scores f32, beams
     int32, tokens int32), each [B, n_out]; (-inf, -1, -1) where candidates run out."""
-    _chk(logits, torch.float32, "logits")
-    _chk(scores, torch.float32, "scores")
-    if scores.dim() != 2:
+    if logits.dtype is not torch.float32 or scores.dtype is not torch.float32:
+        raise TypeError(f"logits and scores must be torch.float32, got {logits.dtype} and {scores.dtype}")
+    if len(scores.shape) != 2:
         raise ValueError("scores must be [B, beams]")
     B, W = scores.shape
     V = logits.shape[-1]
     if logits.numel() != B * W * V:
         raise ValueError(f"logits must hold {B} x {W} rows, got {list(logits.shape)}")
+    if not (logits.is_contiguous() and scores.is_contiguous()):
+        raise ValueError("logits and scores must be contiguous")
     ctx = _ctx(logits)
     _same_device(logits, scores, workspace)
+    n_out = int(n_out)
     if workspace is None:
         workspace = beam_select_workspace(B, W, V, n_out, logits.device)
-    dev = logits.device
-    n_out = int(n_out)
-    best = torch.empty(B, max(n_out, 0), dtype=torch.float32, device=dev)
+    best = torch.empty(B, max(n_out, 0), dtype=torch.float32, device=logits.device)
     beams = torch.empty_like(best, dtype=torch.int32)
     tokens = torch.empty_like(beams)
     ffi.call("higgs_beam_select", ctx, logits.data_ptr(), scores.data_ptr(), B, W, V, n_out, best.data_ptr(),
-             beams.data_ptr(), tokens.data_ptr(), workspace.data_ptr(), workspace.numel(), _st(dev))
+             beams.data_ptr(), tokens.data_ptr(), workspace.data_ptr(), workspace.numel(), _st(logits.device))
     return best, beams, tokens
 
 

@@ -40,7 +40,7 @@ def check(ps, src, dst):
 
 @pytest.mark.parametrize("kind,layers,Hkv,D", [("bf16", 3, 8, 128), ("bf16", 1, 1, 64), ("bf16", 2, 3, 64),
                                                ("tq4", 3, 8, 128), ("tq4", 2, 1, 128), ("tq4", 5, 3, 128)])
-@pytest.mark.parametrize("n", [1, 5, 63, 64, 65])
+@pytest.mark.parametrize("n", [1, 16, 17, 128, 129])
 def test_kv_copy_pages(kind, layers, Hkv, D, n):
     ids = np.random.default_rng(n).permutation(2 * n + 3)
     check(pools(kind, layers, 2 * n + 3, Hkv, D, seed=n), ids[:n], ids[n:2 * n])
