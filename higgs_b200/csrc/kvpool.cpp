@@ -19,6 +19,7 @@
 #include <algorithm>
 #include <map>
 #include <memory>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -227,6 +228,14 @@ void prune(Node& n, bool is_root) {
   }
 }
 
+void remap(Node& n, const std::map<int32_t, int32_t>& to) {
+  for (int32_t& pg : n.pages) {
+    const auto it = to.find(pg);
+    if (it != to.end()) pg = it->second;
+  }
+  for (auto& kv : n.children) remap(*kv.second, to);
+}
+
 void release_all(higgs_prefix_cache* pc, Node& n) {
   if (n.cached) pool_release(pc->pool, n.pages);
   n.cached = false;
@@ -303,6 +312,55 @@ extern "C" int higgs_block_pool_refcount(const higgs_block_pool* p, int32_t page
   return p->refcount[page];
 }
 
+extern "C" int higgs_block_pool_fork(higgs_block_pool* p, const int32_t* pages, int n_pages, int length,
+                                     int32_t* pages_out, int32_t* copy_src, int32_t* copy_dst) {
+  const int full = length / kPage, need = full + (length % kPage ? 1 : 0);
+  if (!p || length < 0 || n_pages < need || (need > 0 && (!pages || !pages_out)) || !copy_src || !copy_dst)
+    return fail(HIGGS_ERR_INVALID_ARG, "higgs_block_pool_fork: bad argument");
+  for (int i = 0; i < need; ++i)
+    if (pages[i] >= (int32_t)p->refcount.size() || (pages[i] >= 0 ? p->refcount[pages[i]] <= 0 : i == full))
+      return fail(HIGGS_ERR_INVALID_ARG,
+                  "higgs_block_pool_fork: page " + std::to_string(pages[i]) + " is not allocated");
+  *copy_src = *copy_dst = -1;
+  if (need > full) {
+    int32_t fresh;
+    if (int rc = higgs_block_pool_alloc(p, 1, &fresh)) return rc;
+    *copy_src = pages[full];
+    *copy_dst = fresh;
+  }
+  for (int i = 0; i < full; ++i) {
+    if (pages[i] >= 0) p->refcount[pages[i]]++;
+    pages_out[i] = pages[i];
+  }
+  if (need > full) pages_out[full] = *copy_dst;
+  return HIGGS_OK;
+}
+
+extern "C" int higgs_block_pool_compact(higgs_block_pool* p, int max_moves, int32_t* src, int32_t* dst,
+                                        int* n_moves) try {
+  if (!p || max_moves < 0 || (max_moves > 0 && (!src || !dst)) || !n_moves)
+    return fail(HIGGS_ERR_INVALID_ARG, "higgs_block_pool_compact: bad argument");
+  const int32_t pages = (int32_t)p->refcount.size();
+  std::vector<int32_t> free_list;
+  free_list.reserve((size_t)pages);
+  int n = 0;
+  for (int32_t lo = 0, hi = pages - 1; n < max_moves; ++n) {
+    while (lo < pages && p->refcount[lo] > 0) ++lo;
+    while (hi >= 0 && p->refcount[hi] <= 0) --hi;
+    if (lo >= hi) break;
+    src[n] = hi;
+    dst[n] = lo;
+    std::swap(p->refcount[lo], p->refcount[hi]);
+  }
+  for (int32_t i = pages - 1; i >= 0; --i)  // the lowest free page is handed out first
+    if (p->refcount[i] <= 0) free_list.push_back(i);
+  p->free_list.swap(free_list);
+  *n_moves = n;
+  return HIGGS_OK;
+} catch (const std::bad_alloc&) {
+  return fail(HIGGS_ERR_STATE, "higgs_block_pool_compact: out of host memory");
+}
+
 // ---------------------------------------------------------------------------
 // prefix cache
 // ---------------------------------------------------------------------------
@@ -377,4 +435,15 @@ extern "C" int higgs_prefix_cache_store(higgs_prefix_cache* pc, const int32_t* t
     }
   }
   return HIGGS_OK;
+}
+
+extern "C" int higgs_prefix_cache_remap(higgs_prefix_cache* pc, const int32_t* src, const int32_t* dst, int n) try {
+  if (!pc || n < 0 || (n > 0 && (!src || !dst)))
+    return fail(HIGGS_ERR_INVALID_ARG, "higgs_prefix_cache_remap: bad argument");
+  std::map<int32_t, int32_t> to;
+  for (int i = 0; i < n; ++i) to[src[i]] = dst[i];
+  remap(pc->root, to);
+  return HIGGS_OK;
+} catch (const std::bad_alloc&) {
+  return fail(HIGGS_ERR_STATE, "higgs_prefix_cache_remap: out of host memory");
 }

@@ -78,6 +78,7 @@ struct higgs_model {
   void* v_scales = nullptr;
   const int8_t* signs = nullptr;
   int64_t num_pages = 0;
+  int window = 0, sinks = 0;  // attention window (0 = none) and its first visible keys
   higgs_comm* comm = nullptr;  // tensor-parallel shard: sums / argmax over ranks
 };
 
@@ -95,7 +96,7 @@ size_t align_up(size_t v) { return (v + kAlign - 1) / kAlign * kAlign; }
 
 struct WsLayout {
   size_t h, h2, x, qkv, q, attn, act, xl, logits, moe_rl, moe_idx, moe_sc, moe_plan, moe_act, moe_y,
-      tp_part, tp_keys, tc_ws, tc_ws_bytes, chain_bar, attn_ws, total;
+      tp_part, tp_keys, tc_ws, tc_ws_bytes, chain_bar, win_ws, win_ws_bytes, attn_ws, total;
 };
 
 int head_rows(const higgs_model_config& c) { return c.tp_world > 1 ? c.head_rows : c.vocab; }
@@ -103,7 +104,8 @@ int head_rows(const higgs_model_config& c) { return c.tp_world > 1 ? c.head_rows
 
 
 
-WsLayout layout(const higgs_model_config& c, int B, int Lq, int max_seq_len, bool last_only) {
+WsLayout layout(const higgs_model* m, int B, int Lq, int max_seq_len, bool last_only) {
+  const higgs_model_config& c = m->cfg;
   const size_t T = (size_t)B * Lq;
   const size_t rows_lm = last_only ? (size_t)B : T;
   const int D = c.head_dim;
@@ -148,6 +150,11 @@ WsLayout layout(const higgs_model_config& c, int B, int Lq, int max_seq_len, boo
   }
   // decode-chain barrier counters, kChainMaxPhases per layer (zero between launches)
   L.chain_bar = take((size_t)c.layers * kChainMaxPhases * kChainBarWords * 4);
+  if (m->window > 0) {
+    L.win_ws_bytes =
+        higgs_window_attention_workspace_size(B, Lq, c.heads, c.kv_heads, D, max_seq_len, m->window, m->sinks);
+    L.win_ws = take(L.win_ws_bytes);
+  }
   const size_t aws = higgs_paged_attention_workspace_size(B, Lq, c.heads, c.kv_heads, D, max_seq_len);
   L.attn_ws = take(aws);
   L.total = off;
@@ -224,7 +231,7 @@ int forward_impl(higgs_model* m, const higgs_forward_args* f, cudaStream_t st) {
   const int D = c.head_dim, H = c.hidden;
   const bool tq = c.kv_mode == HIGGS_KV_TQ4;
   const int n_layers = f->n_layers > 0 ? f->n_layers : c.layers;
-  const WsLayout L = layout(c, B, Lq, f->max_seq_len, f->last_only != 0);
+  const WsLayout L = layout(m, B, Lq, f->max_seq_len, f->last_only != 0);
   if (f->workspace_bytes < L.total)
     return fail(HIGGS_ERR_WORKSPACE, "higgs_model_forward: workspace too small (need " +
                                          std::to_string(L.total) + " bytes)");
@@ -370,7 +377,7 @@ int forward_impl(higgs_model* m, const higgs_forward_args* f, cudaStream_t st) {
   for (int li = 0; li < n_layers; ++li) {
     const LayerW& Lw = m->layers[li];
     L2Prefetch next_pf{};
-    const bool attn_fused = !tq && (c.heads / c.kv_heads) * Lq <= 32;
+    const bool attn_fused = !tq && !m->window && (c.heads / c.kv_heads) * Lq <= 32;
     if (!qkv_ready) {
       if (!fuse) {
         rc = higgs_rmsnorm(m->ctx, h, nullptr, T, H, Lw.ln_in, c.rms_eps, x, nullptr, st);
@@ -434,7 +441,7 @@ int forward_impl(higgs_model* m, const higgs_forward_args* f, cudaStream_t st) {
           HIGGS_PAGE_SIZE * 64, f->block_table, f->max_blocks, f->seq_lens, f->max_seq_len,
           m->signs, scale, attn, aws, aws_bytes, st);
       if (rc) return rc;
-    } else if ((c.heads / c.kv_heads) * Lq <= 32) {
+    } else if (attn_fused) {
       // decode / verify: norm + RoPE + append + attention in one kernel
       uint16_t* kc = (uint16_t*)m->k_pool + li * kv_layer_elems;
       uint16_t* vc = (uint16_t*)m->v_pool + li * kv_layer_elems;
@@ -453,7 +460,13 @@ int forward_impl(higgs_model* m, const higgs_forward_args* f, cudaStream_t st) {
                                       (int64_t)c.kv_heads * HIGGS_PAGE_SIZE * D,
                                       (int64_t)HIGGS_PAGE_SIZE * D, q, st);
       if (rc) return rc;
-      rc = higgs_paged_attention(m->ctx, q, B, Lq, c.heads, c.kv_heads, D, kc, vc,
+      if (m->window)
+        rc = higgs_window_attention(m->ctx, q, B, Lq, c.heads, c.kv_heads, D, kc, vc,
+                                    (int64_t)c.kv_heads * HIGGS_PAGE_SIZE * D, (int64_t)HIGGS_PAGE_SIZE * D,
+                                    f->block_table, f->max_blocks, f->seq_lens, f->max_seq_len, m->window,
+                                    m->sinks, scale, attn, ws + L.win_ws, L.win_ws_bytes, st);
+      else
+        rc = higgs_paged_attention(m->ctx, q, B, Lq, c.heads, c.kv_heads, D, kc, vc,
                                  (int64_t)c.kv_heads * HIGGS_PAGE_SIZE * D,
                                  (int64_t)HIGGS_PAGE_SIZE * D, f->block_table, f->max_blocks,
                                  f->seq_lens, f->max_seq_len, scale, attn, aws, aws_bytes, st);
@@ -804,6 +817,15 @@ extern "C" int higgs_model_set_comm(higgs_model* m, higgs_comm* comm) {
   return HIGGS_OK;
 }
 
+extern "C" int higgs_model_set_attention_window(higgs_model* m, int window, int sinks) {
+  HG_CHECK_ARG(m && window >= 0 && sinks >= 0, "higgs_model_set_attention_window: bad argument");
+  HG_CHECK_ARG(window == 0 || m->cfg.kv_mode == HIGGS_KV_BF16,
+               "higgs_model_set_attention_window: TurboQuant pages have no windowed attention");
+  m->window = window;
+  m->sinks = sinks;
+  return HIGGS_OK;
+}
+
 extern "C" int higgs_model_set_kv_cache(higgs_model* m, void* k_pool, void* v_pool,
                                         int64_t num_pages) {
   HG_CHECK_ARG(m && k_pool && v_pool && num_pages > 0, "higgs_model_set_kv_cache: bad argument");
@@ -834,7 +856,7 @@ extern "C" int higgs_model_set_kv_cache_tq4(higgs_model* m, uint8_t* k_codes, vo
 extern "C" size_t higgs_model_workspace_size(const higgs_model* m, int B, int Lq, int max_seq_len,
                                              int last_only) {
   if (!m || B <= 0 || Lq <= 0) return 0;
-  return layout(m->cfg, B, Lq, max_seq_len, last_only != 0).total;
+  return layout(m, B, Lq, max_seq_len, last_only != 0).total;
 }
 
 extern "C" int higgs_model_forward(higgs_model* m, const higgs_forward_args* f, void* stream) {

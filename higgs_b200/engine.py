@@ -45,6 +45,7 @@ class Sequence:
     last_token: int = -1
     generated: list = dataclasses.field(default_factory=list)
     prefix_hit: int = 0
+    trimmed: int = 0  # leading pages already looked at by Engine._trim
 
 
 class _DecodeGraph:
@@ -135,13 +136,73 @@ class Engine:
             seq.pages.extend(self.pool.alloc(need).tolist())
 
     def release(self, seq: Sequence):
-        if seq.pages:
-            self.pool.release(np.array(seq.pages, np.int32))
+        live = [p for p in seq.pages if p >= 0]
+        if live:
+            self.pool.release(np.array(live, np.int32))
         seq.pages = []
+
+    def _trim(self, seq: Sequence):
+        """Gives up the pages that no later token sees: wholly behind the model's attention window
+        and past its sinks.  Their entries become -1 (the attention does not look them up)."""
+        m = self.model
+        if not m.attn_window:
+            return
+        first = -(-min(m.attn_sinks, seq.length) // PAGE)  # pages of sinks stay
+        last = max(0, seq.length - m.attn_window + 1) // PAGE  # pages before this one are behind
+        gone = [i for i in range(max(first, seq.trimmed), last) if seq.pages[i] >= 0]
+        if gone:
+            self.pool.release(np.array([seq.pages[i] for i in gone], np.int32))
+            for i in gone:
+                seq.pages[i] = -1
+        seq.trimmed = max(seq.trimmed, last)
+
+    def fork(self, seq: Sequence, n: int = 1) -> list[Sequence]:
+        """n further sequences that continue `seq`: whole pages are shared, the partly filled last
+        page is copied for each."""
+        out, src, dst = [], [], []
+        try:
+            for _ in range(n):
+                out.append(self._fork_pages(seq, src, dst))
+        except Exception:
+            for s in out:
+                self.release(s)
+            raise
+        self._copy_pages(src, dst)
+        return out
+
+    def _fork_pages(self, seq: Sequence, src: list, dst: list) -> Sequence:
+        """A second owner of the sequence; the page to copy is added to src and dst."""
+        pages, copy = self.pool.fork(seq.pages, seq.length)
+        if copy is not None:
+            src.append(copy[0])
+            dst.append(copy[1])
+        return dataclasses.replace(seq, pages=pages.tolist(), generated=list(seq.generated))
+
+    def _copy_pages(self, src, dst):
+        from . import ops
+        if len(src):
+            ops.kv_copy_pages(self.model.kv_pools, np.array(src, np.int32), np.array(dst, np.int32))
+
+    def compact(self, seqs: list[Sequence], max_moves: int | None = None) -> int:
+        """Packs the pool's allocated pages into its lowest ids; `seqs` must be all sequences that
+        own pages.  Returns the number of pages moved."""
+        src, dst = self.pool.compact(max_moves)
+        if not src.size:
+            return 0
+        self._copy_pages(src, dst)
+        to = dict(zip(src.tolist(), dst.tolist()))
+        for s in seqs:
+            s.pages = [to.get(p, p) for p in s.pages]
+        self.prefix.remap(src, dst)
+        return int(src.size)
 
     # ---- prefill -------------------------------------------------------------------------
     def prefill(self, prompt, use_prefix: bool = True) -> Sequence:
         """Run the prompt (after any cached prefix) and sample the first token greedily."""
+        return self._prefill(prompt, use_prefix, self.keep_logits)[0]
+
+    def _prefill(self, prompt, use_prefix: bool, want_logits: bool):
+        """prefill, and the last token's logits [1, V] on the device (None unless wanted)."""
         prompt = np.ascontiguousarray(prompt, dtype=np.int32)
         if prompt.size + 1 > self.max_seq_len:
             raise ValueError("prompt longer than max_seq_len")
@@ -164,14 +225,14 @@ class Engine:
             torch.from_numpy(new.reshape(1, n)).to(dev), torch.from_numpy(pos.reshape(1, n)).to(dev),
             torch.from_numpy(slots.reshape(1, n)).to(dev), torch.from_numpy(bt).to(dev),
             torch.tensor([prompt.size], dtype=torch.int32, device=dev), self.max_seq_len,
-            last_only=True, want_logits=self.keep_logits)
+            last_only=True, want_logits=want_logits)
         seq.length = prompt.size
         seq.last_token = int(am.cpu()[0])
         if self.keep_logits:
             seq.first_logits = logits.cpu().numpy()[0]
         if use_prefix:
             self.prefix.store(prompt, np.array(seq.pages, np.int32))
-        return seq
+        return seq, logits
 
     # ---- decode ----------------------------------------------------------------------------
     def _graph_for(self, B: int) -> _DecodeGraph:
@@ -190,6 +251,7 @@ class Engine:
         bt_dirty = first
         for b, s in enumerate(seqs):
             before = len(s.pages)
+            self._trim(s)
             self._ensure_pages(s, s.length + 1)
             if len(s.pages) != before or first:
                 g.bt_host[b, :len(s.pages)] = s.pages
@@ -329,6 +391,98 @@ class Engine:
         for s in seqs:
             self.release(s)
         return np.concatenate([first, rest], axis=1)
+
+
+    def generate_beam(self, prompt, beams: int, max_new_tokens: int, eos_token_id: int | None = None,
+                      length_penalty: float = 1.0, use_prefix: bool = True):
+        """Beam search from one prompt: the `beams` best continuations of at most max_new_tokens
+        tokens as (list of token arrays, scores f64), best first; an array ends with eos_token_id
+        where that ended it.  A score is the sum of the tokens' log-probabilities over (number of
+        tokens) ** length_penalty.
+
+        Each step selects 2 * beams candidates on the device (higgs_beam_select): enough for
+        `beams` that go on, however many end.  A parent's first child keeps its pages, further
+        children share its whole pages and get a copy of the last one (one higgs_kv_copy_pages
+        call for all).  The search stops when `beams` hypotheses have ended and no live one can
+        still beat the worst of them."""
+        from . import ops
+        if self.model.tp:
+            raise NotImplementedError("beam search over vocabulary shards")
+        if beams < 1 or beams > 16:
+            raise ValueError("beams must be 1 to 16")
+        if max_new_tokens < 1 or len(prompt) + max_new_tokens > self.max_seq_len:
+            raise ValueError("max_new_tokens must be at least 1 and fit max_seq_len behind the prompt")
+        dev, V, n = self.model.device, self.model.args.vocab_size, 2 * beams
+        seq, logits = self._prefill(prompt, use_prefix, True)
+        seqs, total = [seq], [0.0]  # live hypotheses, best first, and their log-probabilities
+        done: list[tuple[float, list]] = []  # (score, tokens), best first
+        ws: dict[int, torch.Tensor] = {}
+        try:
+            for step in range(max_new_tokens):
+                W = len(seqs)
+                if step:
+                    g = self._graph_for_logits(W)
+                    self.stage_step(seqs, g, first=True)
+                    g.run()
+                    logits = g.logits
+                if W not in ws:
+                    ws[W] = ops.beam_select_workspace(1, W, V, n, dev)
+                best, par, tok = ops.beam_select(logits, torch.tensor([total], dtype=torch.float32).to(dev), n,
+                                                 workspace=ws[W])
+                best, par, tok = (t.cpu().numpy()[0] for t in (best, par, tok))
+                chosen = []  # (parent, token, log-probability) that go on
+                for s, p, t in zip(best.tolist(), par.tolist(), tok.tolist()):
+                    if p < 0 or len(chosen) == beams:
+                        break
+                    if eos_token_id is not None and t == eos_token_id:
+                        done.append((s / (step + 1) ** length_penalty, seqs[p].generated + [t]))
+                    else:
+                        chosen.append((p, t, s))
+                done = sorted(done, key=lambda d: -d[0])[:beams]
+                last = step + 1 == max_new_tokens or not chosen
+                if len(done) == beams and chosen:
+                    # the best that a live hypothesis can still score: no further loss, at the more
+                    # favourable of the lengths it may end with
+                    ahead = max(chosen[0][2] / k ** length_penalty for k in (step + 1, max_new_tokens))
+                    last = last or ahead <= done[-1][0]
+                if last:
+                    live = [(s / (step + 1) ** length_penalty, seqs[p].generated + [t]) for p, t, s in chosen]
+                    done = sorted(done + live, key=lambda d: -d[0])[:beams]
+                    break
+                seqs, total = self._reorder(seqs, chosen), [s for _, _, s in chosen]
+        finally:
+            for s in seqs:
+                self.release(s)
+        return [np.array(t, np.int32) for _, t in done], np.array([s for s, _ in done])
+
+    def _reorder(self, seqs: list[Sequence], chosen) -> list[Sequence]:
+        """The sequences of the chosen (parent, token, ...): each parent's first child takes over
+        its pages, the others fork them; parents without a child are released."""
+        children = [0] * len(seqs)
+        for c in chosen:
+            children[c[0]] += 1
+        for s, k in zip(seqs, children):
+            if not k:
+                self.release(s)
+        forks, src, dst = [], [], []
+        try:
+            for s, k in zip(seqs, children):
+                forks.append([s] if k else [])
+                for _ in range(k - 1):
+                    forks[-1].append(self._fork_pages(s, src, dst))
+        except Exception:
+            for own in forks:
+                for s in own[1:]:
+                    self.release(s)
+            raise
+        self._copy_pages(src, dst)
+        out = []
+        for c in chosen:
+            s = forks[c[0]].pop(0)
+            s.last_token = c[1]
+            s.generated.append(c[1])
+            out.append(s)
+        return out
 
 
 class SpecDecoder:

@@ -79,6 +79,7 @@ SIGNATURES: dict[str, tuple] = {
     "higgs_model_set_tensor": (I, [P, ctypes.c_char_p, P, I, ctypes.POINTER(I64), I]),
     "higgs_model_finalize": (I, [P]),
     "higgs_model_destroy": (I, [P]),
+    "higgs_model_set_attention_window": (I, [P, I, I]),
     "higgs_model_set_kv_cache": (I, [P, P, P, I64]),
     "higgs_model_set_kv_cache_tq4": (I, [P, P, P, P, P, I64, P]),
     "higgs_model_workspace_size": (SZ, [P, I, I, I, I]),
@@ -94,6 +95,9 @@ SIGNATURES: dict[str, tuple] = {
     "higgs_block_pool_retain": (I, [P, P, I]),
     "higgs_block_pool_release": (I, [P, P, I]),
     "higgs_block_pool_refcount": (I, [P, ctypes.c_int32]),
+    "higgs_block_pool_fork": (I, [P, P, I, I, P, P, P]),
+    "higgs_block_pool_compact": (I, [P, I, P, P, ctypes.POINTER(I)]),
+    "higgs_prefix_cache_remap": (I, [P, P, P, I]),
     "higgs_prefix_cache_create": (I, [P, I, ctypes.POINTER(P)]),
     "higgs_prefix_cache_destroy": (I, [P]),
     "higgs_prefix_cache_len": (I, [P]),

@@ -50,6 +50,25 @@ class BlockPool:
     def refcount(self, page: int) -> int:
         return int(ffi.load().higgs_block_pool_refcount(self.handle, page))
 
+    def fork(self, pages, length: int) -> tuple[np.ndarray, tuple[int, int] | None]:
+        """(pages of a second owner of the sequence, the (source, destination) pair of pages to copy
+        or None): whole pages are shared, a partly filled last one is replaced by a fresh one."""
+        p = np.ascontiguousarray(pages, dtype=np.int32)
+        out = np.empty(-(-max(length, 0) // PAGE), np.int32)
+        pair = np.empty(2, np.int32)
+        ffi.call("higgs_block_pool_fork", self.handle, _i32p(p), p.size, length, _i32p(out), _i32p(pair),
+                 _i32p(pair[1:]))
+        return out, None if pair[0] < 0 else (int(pair[0]), int(pair[1]))
+
+    def compact(self, max_moves: int | None = None) -> tuple[np.ndarray, np.ndarray]:
+        """Packs allocated pages into the lowest ids; the moves (sources, destinations), whose
+        pages the caller copies and renames."""
+        m = self.num_pages if max_moves is None else max_moves
+        moves = np.empty((2, max(m, 1)), np.int32)
+        n = ctypes.c_int(0)
+        ffi.call("higgs_block_pool_compact", self.handle, m, _i32p(moves[0]), _i32p(moves[1]), ctypes.byref(n))
+        return moves[0, :n.value].copy(), moves[1, :n.value].copy()
+
 
 class PrefixCache:
     """PrefixCache (prompt_cache.rs:41-311) over whole KV pages."""
@@ -85,3 +104,11 @@ class PrefixCache:
         t = np.ascontiguousarray(tokens, dtype=np.int32)
         p = np.ascontiguousarray(pages, dtype=np.int32)
         ffi.call("higgs_prefix_cache_store", self.handle, _i32p(t), t.size, _i32p(p), p.size)
+
+    def remap(self, src, dst) -> None:
+        """Renames pages src[i] -> dst[i] in every entry (after BlockPool.compact)."""
+        s = np.ascontiguousarray(src, dtype=np.int32)
+        d = np.ascontiguousarray(dst, dtype=np.int32)
+        if s.size != d.size:
+            raise ValueError("remap: lists of different lengths")
+        ffi.call("higgs_prefix_cache_remap", self.handle, _i32p(s), _i32p(d), s.size)

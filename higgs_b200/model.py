@@ -321,10 +321,13 @@ class Model:
 
     def __init__(self, args: ModelArgs, weights: dict[str, torch.Tensor], num_pages: int,
                  kv_mode: str = "bf16", device="cuda:0", signs: np.ndarray | None = None,
-                 tp: TPGroup | None = None):
+                 tp: TPGroup | None = None, attn_window: int = 0, attn_sinks: int = 0):
         """With `tp`, `weights` are this rank's shard (shard_weights) and the model is one
-        rank of a tensor-parallel group: greedy tokens are identical on every rank."""
+        rank of a tensor-parallel group: greedy tokens are identical on every rank.  With
+        `attn_window`, every layer attends to the last attn_window keys and the first
+        attn_sinks ones (bf16 pages only)."""
         self.args = args
+        self.attn_window, self.attn_sinks = int(attn_window), int(attn_sinks)
         self.device = torch.device(device)
         self.weights = weights
         self.kv_mode = kv_mode
@@ -369,7 +372,14 @@ class Model:
             self.v_pool = torch.zeros_like(self.k_pool)
             ffi.call("higgs_model_set_kv_cache", self.handle, self.k_pool.data_ptr(),
                      self.v_pool.data_ptr(), num_pages)
+        if self.attn_window or self.attn_sinks:
+            ffi.call("higgs_model_set_attention_window", self.handle, self.attn_window, self.attn_sinks)
         self._ws: dict[tuple, torch.Tensor] = {}
+
+    @property
+    def kv_pools(self) -> list[torch.Tensor]:
+        """The cache's tensors [layers, num_pages, ...] (what ops.kv_copy_pages takes)."""
+        return [self.k_pool, self.v_pool] + ([self.k_scales, self.v_scales] if self.kv_mode == "tq4" else [])
 
     def __del__(self):
         try:

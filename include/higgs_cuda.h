@@ -689,6 +689,12 @@ int higgs_model_set_kv_cache_tq4(higgs_model* m, uint8_t* k_codes, void* k_scale
                                  uint8_t* v_codes, void* v_scales, int64_t num_pages,
                                  const int8_t* signs);
 
+/* Every layer attends through a window of the last `window` keys and the first `sinks`
+ * keys (higgs_window_attention); window 0 (the default) is plain causal attention.  Set
+ * it before the first higgs_model_workspace_size / forward / capture: the workspace
+ * depends on it.  bf16 pages only. */
+int higgs_model_set_attention_window(higgs_model* m, int window, int sinks);
+
 /* Bytes of scratch higgs_model_forward needs for (B, Lq, max_seq_len, last_only).
  * The workspace must be zero-filled before its first use; every forward leaves
  * its counters (attention splits, decode-chain barriers) zeroed again. */
@@ -724,6 +730,21 @@ int higgs_block_pool_alloc(higgs_block_pool* pool, int n, int32_t* pages);
 int higgs_block_pool_retain(higgs_block_pool* pool, const int32_t* pages, int n);
 int higgs_block_pool_release(higgs_block_pool* pool, const int32_t* pages, int n);
 int higgs_block_pool_refcount(const higgs_block_pool* pool, int32_t page);
+/* A second owner for a sequence of `length` tokens in `pages` (entries < 0: pages given up
+ * behind an attention window): its whole pages gain a reference, and a partly filled last
+ * page -- which both owners would write -- is replaced by a fresh one.  pages_out gets the
+ * new owner's ceil(length / 16) entries; *copy_src / *copy_dst the page to copy
+ * (higgs_kv_copy_pages), or -1 when length is a multiple of 16.  Nothing is changed when no
+ * page is free (HIGGS_ERR_OUT_OF_PAGES). */
+int higgs_block_pool_fork(higgs_block_pool* pool, const int32_t* pages, int n_pages, int length,
+                          int32_t* pages_out, int32_t* copy_src, int32_t* copy_dst);
+/* Packs the pool: moves at most max_moves allocated pages, highest first, into the lowest
+ * free ids (with their counts) and returns the moves src[i] -> dst[i], *n_moves of them: no
+ * page is in both lists.  With enough moves the allocated pages are then [0, allocated).  The
+ * caller copies the pages (higgs_kv_copy_pages), renames them wherever it keeps them and in
+ * the prefix cache, before any of the ids is used again. */
+int higgs_block_pool_compact(higgs_block_pool* pool, int max_moves, int32_t* src, int32_t* dst,
+                             int* n_moves);
 
 /* PrefixCache (crates/higgs-engine/src/prompt_cache.rs:41-311) over pages:
  * a compressed radix trie of token ids whose entries hold page ids.  Only the
@@ -744,6 +765,9 @@ int higgs_prefix_cache_lookup(higgs_prefix_cache* pc, const int32_t* tokens, int
                               int32_t* pages_out, int max_pages, int* matched_tokens);
 int higgs_prefix_cache_store(higgs_prefix_cache* pc, const int32_t* tokens, int n,
                              const int32_t* pages, int n_pages);
+/* Renames pages src[i] -> dst[i] in every entry, after higgs_block_pool_compact (which
+ * moved their counts). */
+int higgs_prefix_cache_remap(higgs_prefix_cache* pc, const int32_t* src, const int32_t* dst, int n);
 
 /* ---- (f)2: MLX-format safetensors model directories --------------------- */
 

@@ -1,0 +1,172 @@
+"""CPU: forking and packing pages of the pool, renaming them in the prefix cache, and the refusals of
+the device entry points that need no device."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from higgs_b200.ffi import HiggsError
+from higgs_b200.kv import BlockPool, PrefixCache
+
+
+@pytest.mark.parametrize("length", [0, 1, 15, 16, 17, 32, 47, 48])
+def test_fork_shares_whole_pages(length):
+    pool = BlockPool(10)
+    pages = pool.alloc(3)
+    mine, copy = pool.fork(pages, length)
+    full = length // 16
+    assert mine.size == -(-length // 16)
+    assert mine[:full].tolist() == pages[:full].tolist()
+    assert [pool.refcount(int(p)) for p in pages] == [2] * full + [1] * (3 - full)
+    if length % 16:
+        assert copy == (int(pages[full]), int(mine[full])) and copy[1] not in pages.tolist()
+        assert pool.refcount(copy[1]) == 1 and pool.num_free == 6
+    else:
+        assert copy is None and pool.num_free == 7
+    pool.release(mine)
+    pool.release(pages)
+    assert pool.num_free == 10
+
+
+def test_fork_keeps_given_up_pages_and_is_all_or_nothing():
+    pool = BlockPool(4)
+    pages = pool.alloc(4)
+    pool.release(pages[1:2])
+    trimmed = [int(pages[0]), -1, int(pages[2]), int(pages[3])]
+    mine, copy = pool.fork(trimmed, 50)
+    assert mine[1] == -1 and copy[0] == trimmed[3] and copy[1] == int(pages[1])
+    with pytest.raises(HiggsError) as e:
+        pool.fork(trimmed, 50)
+    assert e.value.code == -7
+    assert [pool.refcount(p) for p in trimmed if p >= 0] == [2, 2, 1]
+    for bad, n in (([0, 99], 20), ([0, -1], 20), ([0], 20), ([0, 1], -1)):
+        with pytest.raises(HiggsError):
+            pool.fork(bad, n)
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_compact_packs_pages(seed):
+    rng = np.random.default_rng(seed)
+    n = int(rng.integers(1, 60))
+    pool = BlockPool(n)
+    own = pool.alloc(n)
+    content = {int(p): i for i, p in enumerate(own)}
+    drop = own[rng.random(n) < 0.5]
+    pool.release(drop)
+    live = [int(p) for p in own if p not in drop]
+    for p in live[::3]:
+        pool.retain([p])
+    counts = {p: pool.refcount(p) for p in live}
+    free = pool.num_free
+    src, dst = pool.compact()
+    assert not set(src.tolist()) & set(dst.tolist()) and len(set(dst.tolist())) == dst.size
+    to = dict(zip(src.tolist(), dst.tolist()))
+    moved = {to.get(p, p): content[p] for p in live}
+    assert sorted(moved) == list(range(len(live))) and pool.num_free == free
+    assert all(pool.refcount(to.get(p, p)) == counts[p] for p in live)
+    assert pool.compact()[0].size == 0
+    if free:
+        assert int(pool.alloc(1)[0]) == len(live)  # the lowest free page comes first
+
+
+def test_compact_bounded():
+    pool = BlockPool(10)
+    pages = pool.alloc(10)
+    pool.release(pages[:5])
+    src, dst = pool.compact(2)
+    assert src.tolist() == [9, 8] and dst.tolist() == [0, 1]
+    src, dst = pool.compact()
+    assert src.tolist() == [7, 6, 5] and dst.tolist() == [2, 3, 4]
+
+
+def test_prefix_cache_remap():
+    pool = BlockPool(20)
+    pc = PrefixCache(pool, 4)
+    hole = pool.alloc(4)
+    pages = pool.alloc(3)
+    toks = np.arange(48, dtype=np.int32)
+    pc.store(toks, pages)
+    pool.release(hole)
+    src, dst = pool.compact()
+    pc.remap(src, dst)
+    to = dict(zip(src.tolist(), dst.tolist()))
+    pages = np.array([to.get(int(p), int(p)) for p in pages], np.int32)
+    m, got = pc.lookup(toks)
+    assert m == 48 and got.tolist() == pages.tolist() and sorted(pages.tolist()) == [0, 1, 2]
+    pool.release(got)
+    pool.release(pages)
+    pc.clear()
+    assert pool.num_free == 20
+    with pytest.raises(ValueError):
+        pc.remap([1, 2], [3])
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from higgs_b200 import ffi
+    return ffi.load()
+
+
+def _err(lib):
+    return lib.higgs_last_error().decode()
+
+
+def test_window_attention_arguments_without_device(lib):
+    """Shape and alignment checks come before any CUDA call."""
+    def call(D=128, Hq=32, Hkv=8, B=1, Lq=1, mb=64, msl=1024, w=128, s=4, sc=0.1, q=4096, ps=16384, wsb=1 << 24,
+             ws=4096):
+        p = 4096
+        return lib.higgs_window_attention(p, q, B, Lq, Hq, Hkv, D, p, p, ps, 2048, p, mb, p, msl, w, s,
+                                          ctypes.c_float(sc), p, ws, wsb, None)
+    for kw, why in ((dict(D=96), "D must be"), (dict(w=0), "window >= 1"), (dict(s=-1), "sinks >= 0"),
+                    (dict(Hq=30), "head shape"), (dict(B=0), "head shape"), (dict(Lq=0), "head shape"),
+                    (dict(msl=1025), "block table too short"), (dict(msl=0), "head shape"),
+                    (dict(q=4098), "16-byte aligned"), (dict(ps=16385), "16-byte aligned"),
+                    (dict(ws=4104), "16-byte aligned"), (dict(sc=0.0), "scale"), (dict(sc=float("nan")), "scale"),
+                    (dict(wsb=16), "workspace too small"), (dict(q=None), "null argument")):
+        assert call(**kw) in (-1, -4), kw
+        assert why in _err(lib), (kw, _err(lib))
+
+
+def test_window_attention_workspace_size(lib):
+    f = lib.higgs_window_attention_workspace_size
+    assert f(1, 1, 32, 8, 128, 2048, 1024, 4) > 16384
+    assert f(1, 2048, 32, 8, 128, 4096, 1024, 4) == 16384  # tensor-core tiles: counters only
+    assert f(1, 1, 32, 8, 128, 2048, 2 ** 31 - 1, 2 ** 31 - 1) == f(1, 1, 32, 8, 128, 2048, 2048, 2048)
+    for bad in ((0, 1, 32, 8, 128, 64, 8, 0), (1, 1, 30, 8, 128, 64, 8, 0), (1, 1, 32, 8, 96, 64, 8, 0),
+                (1, 1, 32, 8, 128, 64, 0, 0), (1, 1, 32, 8, 128, 64, 8, -1)):
+        assert f(*bad) == 0
+
+
+def test_beam_select_arguments_without_device(lib):
+    def call(B=1, W=4, V=1000, n=8, ws=4096, wsb=1 << 24, logits=4096):
+        p = 4096
+        return lib.higgs_beam_select(p, logits, p, B, W, V, n, p, p, p, ws, wsb, None)
+    for kw, why in ((dict(B=0), "B 1..1024"), (dict(B=1025), "B 1..1024"), (dict(W=33), "beams 1..32"),
+                    (dict(V=163841), "V 1..163840"), (dict(n=0), "n_out 1..32"), (dict(n=33), "n_out 1..32"),
+                    (dict(ws=4100), "16-byte"), (dict(wsb=4607), "workspace too small"), (dict(logits=None), "null")):
+        assert call(**kw) in (-1, -4), kw
+        assert why in _err(lib), (kw, _err(lib))
+    f = lib.higgs_beam_select_workspace_size
+    assert f(1, 33, 1000, 4) == 0 and f(1, 4, 1000, 4) > 4096 and f(1024, 32, 163840, 32) > 0
+
+
+def test_kv_copy_arguments_without_device(lib):
+    def call(src, dst, base=4096, layers=1, pages=10, ls=16000, ps=1600, pb=1600, n_pools=1):
+        words = (ctypes.c_int64 * 6)(base or 0, layers, pages, ls, ps, pb)
+        s, d = np.array(src, np.int32), np.array(dst, np.int32)
+        return lib.higgs_kv_copy_pages(4096, words, n_pools, s.ctypes.data, d.ctypes.data, s.size, None)
+    assert call([], []) == 0
+    for a, kw, why in ((([1, 2], [3, 3]), {}, "two copies"), (([1, 3], [3, 4]), {}, "also a source"),
+                       (([1], [1]), {}, "also a source"), (([1], [10]), {}, "outside"), (([-1], [1]), {}, "outside"),
+                       (([1], [2]), dict(base=4100), "multiples of 16"), (([1], [2]), dict(pb=1601), "multiples of 16"),
+                       (([1], [2]), dict(ps=1584), "overlap"), (([1], [2]), dict(pages=0), "empty pool"),
+                       (([1], [2]), dict(base=None), "empty pool"), (([1], [2]), dict(n_pools=0), "1 to 8"),
+                       (([1], [2]), dict(n_pools=9), "1 to 8")):
+        assert call(*a, **kw) == -1, (a, kw)
+        assert why in _err(lib), (a, kw, _err(lib))
+
+
+def test_set_attention_window_without_device(lib):
+    assert lib.higgs_model_set_attention_window(None, 16, 0) == -1
+    assert "bad argument" in _err(lib)
