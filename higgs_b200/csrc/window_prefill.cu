@@ -78,6 +78,9 @@ struct WpTile {
   }
   __device__ bool is_sink(int j) const { return j < sink_blocks; }
   __device__ int key(int j) const { return is_sink(j) ? j * kKeys : base + (j - sink_blocks) * kKeys; }
+  __device__ int keys_end(int j) const { return is_sink(j) ? sink_keys : kv_len; }
+  // half blocks of 64 keys that hold any key: 2, or 1 of the last block of either part
+  __device__ int halves(int j) const { return keys_end(j) - key(j) > kHalf ? 2 : 1; }
 };
 
 __device__ __forceinline__ bool wp_wait(uint64_t* bar, unsigned parity, volatile int* abort, int* err) {
@@ -126,6 +129,12 @@ __device__ __forceinline__ uint32_t elect_lane() {
 // tcgen05 instructions of the elected lane in code that the whole warp runs: operands that are the
 // same for all lanes then sit in uniform registers, which these instructions take, and each costs
 // an issue slot; under a branch of one lane they are moved there first, operand by operand.
+// A descriptor's shared-memory address moved on by `bytes`: the field holds addresses of up to 256
+// KB without a carry.
+__device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t bytes) {
+  return (desc & 0xffffffff00000000ull) | ((uint32_t)desc + (bytes >> 4));
+}
+
 __device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accum) {
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
@@ -230,14 +239,6 @@ __global__ void __launch_bounds__(kWpThreads, 1)
     const uint32_t so = (dc >> 3) * (kKeys * 128) + k0 * 128 + (((dc & 7) ^ (k0 & 7)) << 4);
     const uint32_t q_addr = smem_u32(qs) + so, ring_addr = smem_u32(ring) + so;
     int n = 0;  // ring tiles issued
-    // this warp's part of a tile is in shared memory: generic writes before the tensor core's reads
-    auto arrive_after_copies = [&](uint64_t* bar) {
-      cp_async_commit();
-      cp_async_wait<0>();
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar);
-    };
     for (int k = 0;; ++k) {
       if (lt == 0) {
         int i = k == 0 ? blockIdx.x : gridDim.x + atomicAdd(a.counters, 1);
@@ -255,60 +256,71 @@ __global__ void __launch_bounds__(kWpThreads, 1)
       const int32_t* bt = a.bt + (size_t)T.b * a.max_blocks;
       const size_t col = (size_t)T.h * a.head_stride + dc * 8;
       for (int j = 0; j < max(1, T.blocks); ++j) {
-        if (j < T.blocks) {
-          const int kb = T.key(j);
-          // a block all of whose keys are seen by some row comes by TMA, a box per page and 64 of d
-          const bool whole = T.is_sink(j) ? kb + kKeys <= T.sink_keys
-                                          : kb + kKeys <= T.kv_len && (kb >= T.lo || kb + kKeys <= a.sinks);
-          if (whole) {
-            const int box = lane % (8 * (D / 64)), page = bt[(kb >> 4) + box / (D / 64)], panel = box % (D / 64);
+        const int kb = T.key(j);
+        // a block all of whose keys are seen by some row comes by TMA, a box per page and 64 of d
+        const bool whole = kb + kKeys <= T.keys_end(j) && (T.is_sink(j) || kb >= T.lo || kb + kKeys <= a.sinks);
+        const int n0 = n;
+        if (j < T.blocks && whole) {
+          const int box = lane % (8 * (D / 64)), page = bt[(kb >> 4) + box / (D / 64)], panel = box % (D / 64);
 #pragma unroll
-            for (int v = 0; v < 2; ++v, ++n) {
-              const int s = n % SLOTS;
-              if (n >= SLOTS) wp_wait(&kv_empty[s], ((n / SLOTS) - 1) & 1, abort, a.err);
-              __syncwarp();
-              if (lane == 0) {
-                if (warp == 8)
-                  mbar_arrive_expect_tx(&kv_full[s], kTile);
-                else
-                  mbar_arrive(&kv_full[s]);
-              }
-              __syncwarp();
-              if (warp == 8 && lane < 8 * (D / 64))
-                tma_page(smem_u32(ring) + s * kTile + panel * (kKeys * 128) + (box / (D / 64)) * 2048,
-                         v ? &v_map : &k_map, panel * 64, T.h, page, &kv_full[s]);
+          for (int v = 0; v < 2; ++v, ++n) {
+            const int s = n % SLOTS;
+            if (n >= SLOTS) wp_wait(&kv_empty[s], ((n / SLOTS) - 1) & 1, abort, a.err);
+            __syncwarp();
+            if (lane == 0) {
+              if (warp == 8)
+                mbar_arrive_expect_tx(&kv_full[s], kTile);
+              else
+                mbar_arrive(&kv_full[s]);
             }
-          } else {
-            int64_t off[KPT];  // < 0: a key that no row sees; its page is not looked up, it may be free
+            __syncwarp();
+            if (warp == 8 && lane < 8 * (D / 64))
+              tma_page(smem_u32(ring) + s * kTile + panel * (kKeys * 128) + (box / (D / 64)) * 2048,
+                       v ? &v_map : &k_map, panel * 64, T.h, page, &kv_full[s]);
+          }
+        } else if (j < T.blocks) {
+          int64_t off[KPT];  // < 0: a key that no row sees; its page is not looked up, it may be free
 #pragma unroll
-            for (int q = 0; q < KPT; ++q) {
-              const int kg = kb + k0 + q * KSTEP;
-              const bool ok = T.is_sink(j) ? kg < T.sink_keys : kg < T.kv_len && (kg >= T.lo || kg < a.sinks);
-              off[q] = ok ? (int64_t)bt[kg >> 4] * a.page_stride + (int64_t)col + (kg & 15) * D : -1;
-            }
+          for (int q = 0; q < KPT; ++q) {
+            const int kg = kb + k0 + q * KSTEP;
+            const bool ok = kg < T.keys_end(j) && (T.is_sink(j) || kg >= T.lo || kg < a.sinks);
+            off[q] = ok ? (int64_t)bt[kg >> 4] * a.page_stride + (int64_t)col + (kg & 15) * D : -1;
+          }
 #pragma unroll
-            for (int v = 0; v < 2; ++v, ++n) {
-              const int s = n % SLOTS;
-              if (n >= SLOTS) wp_wait(&kv_empty[s], ((n / SLOTS) - 1) & 1, abort, a.err);
-              const uint16_t* pool = v ? a.vc : a.kc;
+          for (int v = 0; v < 2; ++v, ++n) {
+            const int s = n % SLOTS;
+            if (n >= SLOTS) wp_wait(&kv_empty[s], ((n / SLOTS) - 1) & 1, abort, a.err);
+            const uint16_t* pool = v ? a.vc : a.kc;
 #pragma unroll
-              for (int q = 0; q < KPT; ++q)
-                cp_async16_or_zero(ring_addr + s * kTile + q * KSTEP * 128, pool + (off[q] < 0 ? 0 : off[q]), off[q] >= 0);
-              arrive_after_copies(&kv_full[s]);
-            }
+            for (int q = 0; q < KPT; ++q)
+              cp_async16_or_zero(ring_addr + s * kTile + q * KSTEP * 128, pool + (off[q] < 0 ? 0 : off[q]), off[q] >= 0);
           }
         }
-        if (j > 0) continue;
-        // Q, once the tile before has had its last scores (the first K and V are on their way)
-        if (k >= 1) wp_wait(&q_empty, (k - 1) & 1, abort, a.err);
+        if (j == 0) {
+          // Q, once the tile before has had its last scores (the first K and V are on their way)
+          if (k >= 1) wp_wait(&q_empty, (k - 1) & 1, abort, a.err);
 #pragma unroll 4
-        for (int r = k0; r < kTileRows; r += KSTEP) {
-          const int rr = T.r0 + r, t = rr / a.G, hd = rr - t * a.G;
-          const bool ok = rr < T.r_end;
-          const uint16_t* src = a.q + (((size_t)T.b * a.Lq + (ok ? t : 0)) * a.Hq + T.h * a.G + hd) * D + dc * 8;
-          cp_async16_or_zero(q_addr + (r >> 7) * kTile + ((r & 127) - k0) * 128, src, ok);
+          for (int r = k0; r < kTileRows; r += KSTEP) {
+            const int rr = T.r0 + r, t = rr / a.G, hd = rr - t * a.G;
+            const bool ok = rr < T.r_end;
+            const uint16_t* src = a.q + (((size_t)T.b * a.Lq + (ok ? t : 0)) * a.Hq + T.h * a.G + hd) * D + dc * 8;
+            cp_async16_or_zero(q_addr + (r >> 7) * kTile + ((r & 127) - k0) * 128, src, ok);
+          }
         }
-        arrive_after_copies(&q_full);
+        if (j == 0 || (j < T.blocks && !whole)) {
+          // the copies are in shared memory: generic writes before the tensor core's reads
+          cp_async_commit();
+          cp_async_wait<0>();
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            if (j < T.blocks && !whole) {
+              mbar_arrive(&kv_full[n0 % SLOTS]);
+              mbar_arrive(&kv_full[(n0 + 1) % SLOTS]);
+            }
+            if (j == 0) mbar_arrive(&q_full);
+          }
+        }
       }
     }
   } else if (group == 3) {
@@ -316,52 +328,66 @@ __global__ void __launch_bounds__(kWpThreads, 1)
     const int x = warp - 12;
     if (x < 2) {
       constexpr uint32_t idS = tc_idesc_bf16(kM, kHalf), idO = tc_idesc_bf16(kM, D, true);
-      const uint32_t sq = smem_u32(qs) + x * kTile, sr = smem_u32(ring), lead = elect_lane();
+      const uint32_t lead = elect_lane();
       const uint32_t ub = __shfl_sync(0xffffffffu, tb, 0);
       const uint32_t col_s = ub + x * kM, col_o = ub + COL_O + x * kM;
-      int U = 0;  // half blocks of the CTA's tiles before this one; K of half block u is ring tile u & ~1, V the next
+      const uint64_t q_desc = sw128_desc(smem_u32(qs) + x * kTile), k_desc = sw128_desc(smem_u32(ring));
+      const uint64_t v_desc = sw128_mn_desc(smem_u32(ring), kKeys * 128);
+      // blocks and half blocks of the CTA's tiles so far: K and V of block J are ring tiles 2 J and
+      // 2 J + 1, half block U has buffer U & 1 of tensor memory
+      int J0 = 0, U0 = 0;
       for (int k = 0;; ++k) {
         const int i = next_tile(k, lead != 0);
         if (i >= a.tiles) break;
         const WpTile T(a, i);
-        const int n = 2 * T.blocks;
         wp_wait(&q_full, k & 1, abort, a.err);
-        auto scores = [&](int u) {  // S_u = Q K_u^T, into the buffer that P_{u-2} V_{u-2} has read
-          const int g = U + u, slot = (g & ~1) % SLOTS;
-          if (!(u & 1)) wp_wait(&kv_full[slot], ((g & ~1) / SLOTS) & 1, abort, a.err);
+        int js = 0, hs = 0, us = U0;  // next half block of the scores
+        auto scores = [&] {           // S = Q K^T into the buffer whose weights have been used
+          const int ring_tile = 2 * (J0 + js), slot = ring_tile % SLOTS;
+          if (hs == 0) wp_wait(&kv_full[slot], (ring_tile / SLOTS) & 1, abort, a.err);
           tc_fence_after();
-          const uint32_t sk = sr + slot * kTile + (u & 1) * (kHalf * 128), cs = col_s + (u & 1) * kHalf;
+          const uint64_t kd = desc_at(k_desc, slot * kTile + hs * (kHalf * 128));
+          const uint32_t cs = col_s + (us & 1) * kHalf;
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
-            mma_ss(lead, cs, sw128_desc(sq + (kk >> 2) * (kM * 128) + (kk & 3) * 32),
-                   sw128_desc(sk + (kk >> 2) * (kKeys * 128) + (kk & 3) * 32), idS, kk > 0);
-          commit_if(lead, &s_full[x][u & 1]);
-          if (u & 1) commit_if(lead, &kv_empty[slot]);
-          if (u == n - 1) commit_if(lead, &q_empty);
+            mma_ss(lead, cs, desc_at(q_desc, (kk >> 2) * (kM * 128) + (kk & 3) * 32),
+                   desc_at(kd, (kk >> 2) * (kKeys * 128) + (kk & 3) * 32), idS, kk > 0);
+          commit_if(lead, &s_full[x][us & 1]);
+          ++us;
+          if (++hs < T.halves(js)) return;
+          commit_if(lead, &kv_empty[slot]);
+          hs = 0;
+          if (++js == T.blocks) commit_if(lead, &q_empty);
         };
-        if (n > 0) {
-          scores(0);
-          scores(1);
+        if (T.blocks > 0) {
+          scores();
+          if (js < T.blocks) scores();
         } else if (lead) {
           mbar_arrive(&q_empty);
         }
-        for (int u = 0; u < n; ++u) {
-          const int g = U + u, slot = (g | 1) % SLOTS, phase = (g >> 1) & 1;
-          if (!(u & 1)) wp_wait(&kv_full[slot], ((g | 1) / SLOTS) & 1, abort, a.err);
+        int u = U0;
+        for (int j = 0; j < T.blocks; ++j) {
+          const int ring_tile = 2 * (J0 + j) + 1, slot = ring_tile % SLOTS, nh = T.halves(j);
+          wp_wait(&kv_full[slot], (ring_tile / SLOTS) & 1, abort, a.err);
           // a tile's first product overwrites O: its threads have read the tile's before
-          if (u == 0 && k >= 1) wp_wait(&o_free[x], (k - 1) & 1, abort, a.err);
-          wp_wait(&p_full[x][u & 1], phase, abort, a.err);
-          tc_fence_after();
-          const uint32_t sv = sr + slot * kTile + (u & 1) * (kHalf * 128), cs = col_s + (u & 1) * kHalf;
+          if (j == 0 && k >= 1) wp_wait(&o_free[x], (k - 1) & 1, abort, a.err);
+          for (int h = 0; h < nh; ++h, ++u) {
+            const int phase = (u >> 1) & 1;
+            wp_wait(&p_full[x][u & 1], phase, abort, a.err);
+            tc_fence_after();
+            const uint64_t vd = desc_at(v_desc, slot * kTile + h * (kHalf * 128));
+            const uint32_t cs = col_s + (u & 1) * kHalf;
 #pragma unroll
-          for (int kk = 0; kk < kHalf / 16; ++kk)  // 16 keys = two 8-row atoms = 2 KB
-            mma_ts(lead, col_o, cs + kk * 8, sw128_mn_desc(sv + kk * 2048, kKeys * 128), idO, u > 0 || kk > 0);
-          commit_if(lead, &pv_done[x][u & 1]);
-          if (u & 1) commit_if(lead, &kv_empty[slot]);
-          wp_wait(&pv_done[x][u & 1], phase, abort, a.err);  // (what is next overwrites P)
-          if (u + 2 < n) scores(u + 2);
+            for (int kk = 0; kk < kHalf / 16; ++kk)  // 16 keys = two 8-row atoms = 2 KB
+              mma_ts(lead, col_o, cs + kk * 8, desc_at(vd, kk * 2048), idO, j > 0 || h > 0 || kk > 0);
+            commit_if(lead, &pv_done[x][u & 1]);
+            if (h == nh - 1) commit_if(lead, &kv_empty[slot]);
+            wp_wait(&pv_done[x][u & 1], phase, abort, a.err);  // (what is next overwrites P)
+            if (js < T.blocks) scores();
+          }
         }
-        U += n;
+        J0 += T.blocks;
+        U0 = u;
       }
     }
   } else {
@@ -380,9 +406,9 @@ __global__ void __launch_bounds__(kWpThreads, 1)
       const int pos = valid ? T.first + t : -1;
       float m = -INFINITY;
       float2 l2 = make_float2(0.f, 0.f);
-      const int n = 2 * T.blocks;
-      for (int u = 0; u < n; ++u) {
-        const int buf = u & 1, phase = ((U + u) >> 1) & 1;
+      const int u0 = U;
+      for (int j = 0, h = 0; j < T.blocks; ++U) {
+        const int buf = U & 1, phase = (U >> 1) & 1;
         const uint32_t cs = col_s + buf * kHalf;
         wp_wait(&s_full[x][buf], phase, abort, a.err);
         tc_fence_after();
@@ -390,9 +416,12 @@ __global__ void __launch_bounds__(kWpThreads, 1)
 #pragma unroll
         for (int c = 0; c < kHalf / 16; ++c) tc_ld16(cs + 16 * c, v + 16 * c);
         // key i of the half block is visible iff i <= lim and (i >= low or i < snk)
-        const bool sink = T.is_sink(u >> 1);
-        const int kb = T.key(u >> 1) + buf * kHalf;
-        const int lim = sink ? min(pos, T.sink_keys - 1) - kb : pos - kb;
+        const int kb = T.key(j) + h * kHalf;
+        const int lim = (T.is_sink(j) ? min(pos, T.sink_keys - 1) : pos) - kb;
+        if (++h == T.halves(j)) {
+          h = 0;
+          ++j;
+        }
         const int low = pos - a.window + 1 - kb, snk = a.sinks - kb;
         const bool whole = __all_sync(0xffffffffu, lim >= kHalf - 1 && (low <= 0 || snk >= kHalf));
         tc_wait_ld();
@@ -418,8 +447,8 @@ __global__ void __launch_bounds__(kWpThreads, 1)
           if (grow) m = mx;
           l2.x *= alpha;
           l2.y *= alpha;
-          if (u >= 1) {
-            wp_wait(&pv_done[x][buf ^ 1], ((U + u - 1) >> 1) & 1, abort, a.err);
+          if (U > u0) {
+            wp_wait(&pv_done[x][buf ^ 1], ((U - 1) >> 1) & 1, abort, a.err);
             tc_fence_after();
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
@@ -453,10 +482,9 @@ __global__ void __launch_bounds__(kWpThreads, 1)
         tc_fence_before();
         mbar_arrive(&p_full[x][buf]);
       }
-      U += n;
       // ---- O / l -> bf16 ----
       if (T.blocks > 0) {
-        wp_wait(&pv_done[x][1], ((U - 1) >> 1) & 1, abort, a.err);
+        wp_wait(&pv_done[x][(U - 1) & 1], ((U - 1) >> 1) & 1, abort, a.err);
         tc_fence_after();
       }
       const float l = l2.x + l2.y, inv = l > 0.f ? 1.f / l : 0.f;
