@@ -13,7 +13,7 @@
 //   2     loads Q and, alternating, K_j and V_j of 128 keys into 128-byte-swizzled tiles of a ring: by
 //         TMA, a box per page, or where a block has keys that no row sees (and whose slots may hold
 //         anything: 0 x NaN would be NaN) by 16-byte cp.async with zeros for those
-//   3     one warp per half issues S_u = Q K_u^T two steps ahead, waits for P_u, issues O += P_u V_u
+//   3     per half one warp issues S_u = Q K_u^T, two steps ahead, and one O += P_u V_u
 // S, P and O of both halves fill the 512 columns of tensor memory: per half two buffers of 64 scores
 // and 128 of O.  S_u+1 waits there while the softmax of S_u runs, S_u+2 is issued when P_u V_u is done.
 // Both halves share every K and V tile.
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kWpThreads, 1)
     }
     for (int i = 0; i < kTileRing; ++i) {
       mbar_init(&t_full[i], 1);
-      mbar_init(&t_empty[i], 256 + 2);
+      mbar_init(&t_empty[i], 256 + 4);
     }
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -324,70 +324,61 @@ __global__ void __launch_bounds__(kWpThreads, 1)
       }
     }
   } else if (group == 3) {
-    // ---------------- MMA issue: warp 12 + x for half x ----------------
-    const int x = warp - 12;
-    if (x < 2) {
-      constexpr uint32_t idS = tc_idesc_bf16(kM, kHalf), idO = tc_idesc_bf16(kM, D, true);
-      const uint32_t lead = elect_lane();
-      const uint32_t ub = __shfl_sync(0xffffffffu, tb, 0);
-      const uint32_t col_s = ub + x * kM, col_o = ub + COL_O + x * kM;
-      const uint64_t q_desc = sw128_desc(smem_u32(qs) + x * kTile), k_desc = sw128_desc(smem_u32(ring));
-      const uint64_t v_desc = sw128_mn_desc(smem_u32(ring), kKeys * 128);
-      // blocks and half blocks of the CTA's tiles so far: K and V of block J are ring tiles 2 J and
-      // 2 J + 1, half block U has buffer U & 1 of tensor memory
-      int J0 = 0, U0 = 0;
-      for (int k = 0;; ++k) {
-        const int i = next_tile(k, lead != 0);
-        if (i >= a.tiles) break;
-        const WpTile T(a, i);
+    // ---------------- MMA issue: scores of half x by warp 12 + x, products by warp 14 + x ----------------
+    // (One warp for both holds the next product back behind the next scores.)
+    const int x = warp & 1;
+    const uint32_t lead = elect_lane();
+    const uint32_t ub = __shfl_sync(0xffffffffu, tb, 0);
+    const uint32_t col_s = ub + x * kM, col_o = ub + COL_O + x * kM;
+    // blocks and half blocks of the CTA's tiles so far: K and V of block J are ring tiles 2 J and
+    // 2 J + 1, half block U has buffer U & 1 of tensor memory
+    int J = 0, U = 0;
+    for (int k = 0;; ++k) {
+      const int i = next_tile(k, lead != 0);
+      if (i >= a.tiles) break;
+      const WpTile T(a, i);
+      if (warp < 14) {
+        constexpr uint32_t id = tc_idesc_bf16(kM, kHalf);
+        const uint64_t q_desc = sw128_desc(smem_u32(qs) + x * kTile), k_desc = sw128_desc(smem_u32(ring));
         wp_wait(&q_full, k & 1, abort, a.err);
-        int js = 0, hs = 0, us = U0;  // next half block of the scores
-        auto scores = [&] {           // S = Q K^T into the buffer whose weights have been used
-          const int ring_tile = 2 * (J0 + js), slot = ring_tile % SLOTS;
-          if (hs == 0) wp_wait(&kv_full[slot], (ring_tile / SLOTS) & 1, abort, a.err);
-          tc_fence_after();
-          const uint64_t kd = desc_at(k_desc, slot * kTile + hs * (kHalf * 128));
-          const uint32_t cs = col_s + (us & 1) * kHalf;
+        for (int j = 0; j < T.blocks; ++j, ++J) {
+          const int slot = (2 * J) % SLOTS, nh = T.halves(j);
+          wp_wait(&kv_full[slot], ((2 * J) / SLOTS) & 1, abort, a.err);
+          for (int h = 0; h < nh; ++h, ++U) {
+            // S_u = Q K_u^T into the buffer that holds P_{u-2} until its product is done
+            if (U >= 2) wp_wait(&pv_done[x][U & 1], ((U >> 1) - 1) & 1, abort, a.err);
+            tc_fence_after();
+            const uint64_t kd = desc_at(k_desc, slot * kTile + h * (kHalf * 128));
+            const uint32_t cs = col_s + (U & 1) * kHalf;
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            mma_ss(lead, cs, desc_at(q_desc, (kk >> 2) * (kM * 128) + (kk & 3) * 32),
-                   desc_at(kd, (kk >> 2) * (kKeys * 128) + (kk & 3) * 32), idS, kk > 0);
-          commit_if(lead, &s_full[x][us & 1]);
-          ++us;
-          if (++hs < T.halves(js)) return;
+            for (int kk = 0; kk < D / 16; ++kk)
+              mma_ss(lead, cs, desc_at(q_desc, (kk >> 2) * (kM * 128) + (kk & 3) * 32),
+                     desc_at(kd, (kk >> 2) * (kKeys * 128) + (kk & 3) * 32), id, kk > 0);
+            commit_if(lead, &s_full[x][U & 1]);
+          }
           commit_if(lead, &kv_empty[slot]);
-          hs = 0;
-          if (++js == T.blocks) commit_if(lead, &q_empty);
-        };
-        if (T.blocks > 0) {
-          scores();
-          if (js < T.blocks) scores();
-        } else if (lead) {
-          mbar_arrive(&q_empty);
         }
-        int u = U0;
-        for (int j = 0; j < T.blocks; ++j) {
-          const int ring_tile = 2 * (J0 + j) + 1, slot = ring_tile % SLOTS, nh = T.halves(j);
-          wp_wait(&kv_full[slot], (ring_tile / SLOTS) & 1, abort, a.err);
+        commit_if(lead, &q_empty);  // (at once if the tile had no block)
+      } else {
+        constexpr uint32_t id = tc_idesc_bf16(kM, D, true);
+        const uint64_t v_desc = sw128_mn_desc(smem_u32(ring), kKeys * 128);
+        for (int j = 0; j < T.blocks; ++j, ++J) {
+          const int slot = (2 * J + 1) % SLOTS, nh = T.halves(j);
+          wp_wait(&kv_full[slot], ((2 * J + 1) / SLOTS) & 1, abort, a.err);
           // a tile's first product overwrites O: its threads have read the tile's before
           if (j == 0 && k >= 1) wp_wait(&o_free[x], (k - 1) & 1, abort, a.err);
-          for (int h = 0; h < nh; ++h, ++u) {
-            const int phase = (u >> 1) & 1;
-            wp_wait(&p_full[x][u & 1], phase, abort, a.err);
+          for (int h = 0; h < nh; ++h, ++U) {
+            wp_wait(&p_full[x][U & 1], (U >> 1) & 1, abort, a.err);
             tc_fence_after();
             const uint64_t vd = desc_at(v_desc, slot * kTile + h * (kHalf * 128));
-            const uint32_t cs = col_s + (u & 1) * kHalf;
+            const uint32_t cs = col_s + (U & 1) * kHalf;
 #pragma unroll
             for (int kk = 0; kk < kHalf / 16; ++kk)  // 16 keys = two 8-row atoms = 2 KB
-              mma_ts(lead, col_o, cs + kk * 8, desc_at(vd, kk * 2048), idO, j > 0 || h > 0 || kk > 0);
-            commit_if(lead, &pv_done[x][u & 1]);
-            if (h == nh - 1) commit_if(lead, &kv_empty[slot]);
-            wp_wait(&pv_done[x][u & 1], phase, abort, a.err);  // (what is next overwrites P)
-            if (js < T.blocks) scores();
+              mma_ts(lead, col_o, cs + kk * 8, desc_at(vd, kk * 2048), id, j > 0 || h > 0 || kk > 0);
+            commit_if(lead, &pv_done[x][U & 1]);
           }
+          commit_if(lead, &kv_empty[slot]);
         }
-        J0 += T.blocks;
-        U0 = u;
       }
     }
   } else {
