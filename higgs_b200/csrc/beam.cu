@@ -7,20 +7,27 @@
 //
 // Within a beam the keys are ordered as the logits are, so one pass over a row gives all that is
 // needed of it: the sum of its exponentials and its n largest logits.  A row is cut into rounds of
-// 4096 logits, and the rounds of all rows into equal shares for as many CTAs as are resident at
-// once; a CTA takes its share row by row.  Each warp streams 512 logits of a round, the next
-// round's in flight while it works on these.  It writes the round's maximum and sum of
-// exponentials, and keeps the 32 best keys it has seen, sorted, one per lane.  Logits above the
-// n-th best are rare after the first few rounds; they are collected until there are 32, sorted by a
-// bitonic network and merged.  So the common logit costs a comparison and an exponential, and the
-// worst order (rising logits) only more merges.  The CTA that completes a request's last round
-// joins its lists the same way, on keys in 64 bits: which of two near candidates wins is decided
-// by the difference of two log sums.
+// 4096 logits, and the rounds of all rows into shares for as many CTAs as are resident at once; a
+// CTA takes its share row by row, 16 logits per thread and round, the next round's in flight while
+// it works on these.  Each warp writes the round's maximum and sum of exponentials, and collects
+// the logits that reach a bound to which all eight warps contribute (scan_rounds): after the first
+// rounds they are few, so the common logit costs a comparison and an exponential.  A warp that
+// collects 32 sorts them (a bitonic network) and keeps the best, so no order of the logits needs
+// more room; at the end the CTA's few candidates are ranked by counting those above each.
+//
+// The CTA that completes a request's last round joins its lists, on keys in 64 bits: which of two
+// near candidates wins is decided by the difference of two log sums.  A histogram over the leading
+// bits bounds the n-th best, and what reaches the bound is ranked as above.
 //
 // Keys are unique (value, then index), and the sums of a round depend on its logits alone and are
 // added in the order of the rounds: equal rows give equal keys, and results do not depend on
 // scheduling or on how the rounds are shared out.
-// Bound: HBM, 4 bytes per logit of a beam that is alive.
+//
+// Bound: HBM, 4 bytes per logit of a beam that is alive.  B200: 32 requests x 16 beams x 151936
+// logits, 32 best (311 MB) 73 us = 4.3 TB/s: nine CTAs in ten end their scans 48 to 62 us after the
+// start (equal shares, unequal speeds), and the last one's list and join take 10 more; 8 x 8 beams,
+// 16 best (39 MB) 19.7 us; one request 8.6 us, a chain of launch, one round, list, counter, log
+// sums and join.
 #include <algorithm>
 
 #include "common.cuh"
@@ -96,8 +103,8 @@ __device__ __forceinline__ float logit_of(unsigned long long k) {
 }
 __device__ __forceinline__ int index_of(unsigned long long k) { return (int)(0xffffffffu - (uint32_t)k); }
 
-// lane i of the warp gets the i-th largest of its 32 keys (bitonic network; the loops stay loops,
-// since code that a CTA runs a few times costs more in instruction fetches than in branches)
+// lane i of the warp gets the i-th largest of its 32 keys (bitonic network; it runs rarely, so its
+// loops stay loops)
 template <typename Key>
 __device__ __forceinline__ Key warp_sort(Key k) {
   const int lane = threadIdx.x & 31;
@@ -157,7 +164,7 @@ struct WarpTop {
 
 constexpr int kMaxCand = kBeamWarps * 64;
 constexpr int kMaxLists = 512;    // of a request
-constexpr int kMaxDirect = 2048;  // entries of lists that are bisected as they are
+constexpr int kMaxDirect = 2048;  // entries of lists that are joined directly
 static_assert(kBeamCtasPerSm * 148 + 2 * kMaxBeams <= kMaxLists, "shares that a request's rows can meet");
 template <typename Key>
 struct TopShared {

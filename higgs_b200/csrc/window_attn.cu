@@ -452,8 +452,8 @@ extern "C" int higgs_window_attention(higgs_ctx* ctx, const void* q, int B, int 
                "higgs_window_attention: block table too short (or beyond 2^26 pages)");
   HG_CHECK_ARG((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)workspace) &
                 15) == 0 &&
-                   page_stride % 8 == 0 && head_stride % 8 == 0,
-               "higgs_window_attention: tensors, workspace and strides must be 16-byte aligned");
+                   page_stride % 8 == 0 && head_stride % 8 == 0 && page_stride > 0 && head_stride > 0,
+               "higgs_window_attention: tensors, workspace and (positive) strides must be 16-byte aligned");
   HG_CHECK_ARG(scale > 0.f && scale < INFINITY, "higgs_window_attention: scale must be positive and finite");
   // a window or sinks past the longest sequence are the whole sequence
   window = std::min(window, max_seq_len);

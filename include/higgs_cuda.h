@@ -138,7 +138,8 @@ int higgs_version(void);
  * higgs_paged_attention launches of more than 64 query rows (Hq / Hkv x Lq; G =
  * Hq / Hkv dividing 128, 16-byte aligned buffers and strides) run the tcgen05
  * prefill kernel (128-row tiles of tokens x GQA heads, S and O in tensor memory)
- * instead of the decode kernel's 32-row query chunks.
+ * instead of the decode kernel's 32-row query chunks, and higgs_window_attention's, of any G, one
+ * of 256-row tiles.
  * Unknown names return HIGGS_ERR_INVALID_ARG. */
 int higgs_set_option(const char* name, int value);
 
@@ -384,8 +385,10 @@ int higgs_paged_attention_noalloc(higgs_ctx* ctx, const void* q, int B, int Lq, 
  *   block_table entries: a host may free those pages and leave any value there.  The
  *   slots of hidden keys in other pages may hold anything; K and V of a key that some
  *   query of the call sees must be finite.
- *   D = 64 or 128; Hq / Hkv any whole number.  Base pointers and strides must be
- *   multiples of 16 bytes.  workspace: at least
+ *   D = 64 or 128; Hq / Hkv any whole number.  Base pointers and (positive) strides
+ *   must be multiples of 16 bytes.  More than 64 query rows per kv head, Hq / Hkv * Lq,
+ *   run on the tensor cores (option "attn_prefill_tc"), whose waits are bounded
+ *   (higgs_tc_error).  workspace: at least
  *   higgs_window_attention_workspace_size() bytes (0 for a shape that is refused),
  *   zero-filled before its first use; each call leaves its counters (the first 16384
  *   bytes) zero, so calls of any shapes that follow one another on a stream can share

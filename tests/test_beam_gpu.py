@@ -179,3 +179,47 @@ def test_beam_select_refuses():
         o.beam_select(x, torch.zeros(2, 4, device=DEV), 4)
     with pytest.raises(ValueError):
         o.beam_select(x.cpu(), s, 4)
+
+
+@pytest.mark.parametrize("B,W,V,n", [(1, 16, 151936, 32), (1, 8, 151936, 16), (30, 16, 20000, 32), (445, 1, 9000, 3),
+                                     (6, 32, 4096, 32), (1, 2, 4097, 1)])
+def test_beam_select_shares_and_lists(B, W, V, n):
+    """Shapes of every way the rows are shared out: many lists per request, rows cut across CTAs,
+    more rows than CTAs, single rounds."""
+    x, s = draw(B + W + V, B, W, V)
+    check(x, s, n)
+
+
+def test_beam_select_many_equal_keys_across_lists():
+    """More equal candidates than are ranked directly: every beam alike, few distinct values."""
+    V = 40000
+    row = np.round(np.random.default_rng(1).normal(0, 1, V) * 4).astype(np.float32) / 4
+    x = np.tile(row, (2, 32, 1))
+    check(x, np.full((2, 32), -2.0, np.float32), 32)
+    check(np.zeros((1, 32, V), np.float32), np.zeros((1, 32), np.float32), 32)
+
+
+def test_beam_select_unaligned_logits():
+    """A row length of a multiple of four on a base that is not 16-byte aligned."""
+    x, s = draw(3, 2, 4, 5000)
+    buf = torch.empty(2 * 4 * 5000 + 1, device=DEV)
+    buf[1:] = torch.from_numpy(x).to(DEV).view(-1)
+    got = ops().beam_select(buf[1:].view(8, 5000), torch.from_numpy(s).to(DEV), 8)
+    keys, beams, toks = plain(x, s, 8)
+    assert np.array_equal(got[1].cpu().numpy(), beams) and np.array_equal(got[2].cpu().numpy(), toks)
+    assert (np.abs(got[0].cpu().numpy() - keys) <= tol(keys)).all()
+
+
+def test_beam_select_two_streams():
+    x, s = draw(4, 4, 8, 60000)
+    xt, st = torch.from_numpy(x).to(DEV), torch.from_numpy(s).to(DEV)
+    want = ops().beam_select(xt, st, 16)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(6):
+        for sm in streams:
+            with torch.cuda.stream(sm):
+                got.append(ops().beam_select(xt, st, 16))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))

@@ -128,6 +128,14 @@ def test_window_attention_arguments_without_device(lib):
         assert why in _err(lib), (kw, _err(lib))
 
 
+@pytest.mark.parametrize("page,head", [(-16384, 2048), (0, 2048), (16384, -2048), (16384, 0)])
+def test_window_attention_strides_must_be_positive(lib, page, head):
+    for Lq in (1, 100):  # both kernels
+        assert lib.higgs_window_attention(4096, 4096, 1, Lq, 32, 8, 128, 4096, 4096, page, head, 4096, 64, 4096, 1024,
+                                          128, 4, ctypes.c_float(0.1), 4096, 4096, 1 << 24, None) == -1
+        assert "positive" in _err(lib)
+
+
 def test_window_attention_workspace_size(lib):
     f = lib.higgs_window_attention_workspace_size
     assert f(1, 1, 32, 8, 128, 2048, 1024, 4) > 16384

@@ -129,6 +129,21 @@ def test_window_wider_than_the_cache_is_paged_attention(Lq):
     assert ((a - b).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("case", [(1, 100, 8, 2, 128, [300], 77, 5), (2, 90, 14, 2, 64, [50, 400], 33, 0)],
+                         ids=["d128", "d64"])
+def test_window_attention_many_rows_without_tensor_cores(case):
+    """The 8-row kernel on prompts (option attn_prefill_tc off): its 16-bit weights, many tiles."""
+    from higgs_b200 import ffi
+    q, k, v, bt, sl = make(*case, seed=1)
+    ffi.call("higgs_set_option", b"attn_prefill_tc", 0)
+    try:
+        got = ops().window_attention(q, k, v, bt, sl, max(case[5]), case[6], case[7])
+    finally:
+        ffi.call("higgs_set_option", b"attn_prefill_tc", 1)
+    ref, mag = plain(q, k, v, bt, case[5], case[6], case[7])
+    check(got, ref, mag, 1)
+
+
 @pytest.mark.parametrize("Lq", [1, 4, 100])
 def test_window_attention_strided_caches(Lq):
     """A layer of a [pages, layers, ...] pool, and a head-major pool: pages and heads by strides."""
@@ -217,3 +232,37 @@ def test_window_attention_refuses():
         o.window_attention(q[..., :32].contiguous(), k[..., :32].contiguous(), v[..., :32].contiguous(), *ok[3:])
     with pytest.raises(HiggsError, match="16-byte aligned"):
         o.window_attention(*ok[:5], 40, 16, workspace=torch.zeros(1 << 20, dtype=torch.uint8, device=DEV)[8:])
+
+
+def test_window_attention_scale_and_sharp_scores():
+    """A scale of the caller's, and scores so sharp that one key takes all: the running maximum is
+    raised often."""
+    for Lq, rows in ((1, 4), (150, 600)):
+        q, k, v, bt, sl = make(1, Lq, 8, 2, 128, [700], 500, 4, seed=Lq, qscale=6.0)
+        got = ops().window_attention(q, k, v, bt, sl, 700, 500, 4, scale=0.25)
+        ref, mag = plain(q, k, v, bt, [700], 500, 4, scale=0.25)
+        # scores up to 6 * 4 sigma * sqrt(128) * 0.25 < 2^7 here, so the f32 sums of 128 products are off by
+        # at most 128 * 2^-23 * 2^7 = 2^-9 in weight and norm: 2^-8 of sum w |v|; bf16 weights add 2^-8
+        tol = 2.0 ** -8 * ref.abs() + (2.0 ** -8 + (2.0 ** -8 if rows > 64 else 0)) * mag
+        assert torch.isfinite(got).all() and ((got.double() - ref).abs() <= tol).all()
+        for bad in (0.0, -1.0, math.inf, math.nan):
+            from higgs_b200.ffi import HiggsError
+            with pytest.raises(HiggsError, match="scale"):
+                ops().window_attention(q, k, v, bt, sl, 700, 500, 4, scale=bad)
+
+
+def test_window_attention_default_workspace_on_a_side_stream():
+    """Calls on two streams at once, each with a workspace of its own."""
+    a = make(2, 1, 32, 8, 128, [900, 333], 256, 4, seed=21)
+    b = make(1, 130, 32, 8, 128, [900], 256, 4, seed=22)
+    want = [ops().window_attention(*x, 900, 256, 4) for x in (a, b)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for x, st in zip((a, b), streams):
+            with torch.cuda.stream(st):
+                got.append(ops().window_attention(*x, 900, 256, 4))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert torch.equal(g, want[i % 2])
