@@ -18,7 +18,7 @@
 // and 128 of O.  S_u+1 waits there while the softmax of S_u runs, S_u+2 is issued when P_u V_u is done.
 // Both halves share every K and V tile.
 // Every mbarrier wait is bounded (about 2 s; the first timeout makes the CTA's other waits give up
-// and sets the flag that higgs_tc_error reports).
+// and sets the flag that higgs_tc_error reports; copies and products in flight are then still waited for).
 #include <algorithm>
 
 #include "common.cuh"
@@ -181,7 +181,8 @@ __global__ void __launch_bounds__(kWpThreads, 1)
   __shared__ __align__(8) uint64_t o_free[2];                           // a phase per tile
   __shared__ __align__(8) uint64_t t_full[kTileRing], t_empty[kTileRing];
   __shared__ int tile_ring[kTileRing];
-  __shared__ int loader_tile, abort_flag;
+  __shared__ __align__(8) uint64_t drained;
+  __shared__ int loader_tile, abort_flag, drain_abort;
   __shared__ uint32_t tmem_base;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int group = warp >> 2;
@@ -206,7 +207,8 @@ __global__ void __launch_bounds__(kWpThreads, 1)
       mbar_init(&t_full[i], 1);
       mbar_init(&t_empty[i], 256 + 4);
     }
-    abort_flag = 0;
+    mbar_init(&drained, 4);
+    abort_flag = drain_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
@@ -238,8 +240,8 @@ __global__ void __launch_bounds__(kWpThreads, 1)
     static_assert(KSTEP % 8 == 0, "a thread's rows share their swizzle");
     const uint32_t so = (dc >> 3) * (kKeys * 128) + k0 * 128 + (((dc & 7) ^ (k0 & 7)) << 4);
     const uint32_t q_addr = smem_u32(qs) + so, ring_addr = smem_u32(ring) + so;
-    int n = 0;  // ring tiles issued
-    for (int k = 0;; ++k) {
+    int n = 0, k = 0;  // ring tiles issued; tiles taken
+    for (;; ++k) {
       if (lt == 0) {
         int i = k == 0 ? blockIdx.x : gridDim.x + atomicAdd(a.counters, 1);
         if (i > a.tiles || *abort) i = a.tiles;
@@ -323,6 +325,12 @@ __global__ void __launch_bounds__(kWpThreads, 1)
         }
       }
     }
+    // No copy and no arrival may come after the CTA's shared memory is another's: the ring's copies
+    // (also those that nobody waited for because a wait gave up), then the products' releases.
+    for (int e = max(0, n - SLOTS); e < n; ++e)
+      wp_wait(&kv_full[e % SLOTS], (e / SLOTS) & 1, &drain_abort, a.err);
+    for (int e = max(0, n - SLOTS); e < n; ++e) wp_wait(&kv_empty[e % SLOTS], (e / SLOTS) & 1, abort, a.err);
+    if (k >= 1) wp_wait(&q_empty, (k - 1) & 1, abort, a.err);
   } else if (group == 3) {
     // ---------------- MMA issue: scores of half x by warp 12 + x, products by warp 14 + x ----------------
     // (One warp for both holds the next product back behind the next scores.)
@@ -381,6 +389,9 @@ __global__ void __launch_bounds__(kWpThreads, 1)
         }
       }
     }
+    // tensor memory is given back after the last product, also when a wait gave up before it
+    commit_if(lead, &drained);
+    wp_wait(&drained, 0, &drain_abort, a.err);
   } else {
     // ---------------- softmax: half x, a thread per row ----------------
     const int x = group, r = x * kM + (threadIdx.x & 127);
