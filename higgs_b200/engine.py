@@ -163,11 +163,11 @@ class Engine:
         try:
             for _ in range(n):
                 out.append(self._fork_pages(seq, src, dst))
+            self._copy_pages(src, dst)
         except Exception:
             for s in out:
                 self.release(s)
             raise
-        self._copy_pages(src, dst)
         return out
 
     def _fork_pages(self, seq: Sequence, src: list, dst: list) -> Sequence:
@@ -470,12 +470,12 @@ class Engine:
                 forks.append([s] if k else [])
                 for _ in range(k - 1):
                     forks[-1].append(self._fork_pages(s, src, dst))
+            self._copy_pages(src, dst)
         except Exception:
             for own in forks:
                 for s in own[1:]:
                     self.release(s)
             raise
-        self._copy_pages(src, dst)
         out = []
         for c in chosen:
             s = forks[c[0]].pop(0)

@@ -178,3 +178,28 @@ def test_kv_copy_arguments_without_device(lib):
 def test_set_attention_window_without_device(lib):
     assert lib.higgs_model_set_attention_window(None, 16, 0) == -1
     assert "bad argument" in _err(lib)
+
+
+def _engine_whose_copies_fail(pages=12):
+    from higgs_b200.engine import Engine
+    eng = Engine.__new__(Engine)
+    eng.pool = BlockPool(pages)
+
+    def fail(src, dst):
+        raise RuntimeError("copy")
+    eng._copy_pages = fail
+    return eng
+
+
+def test_forks_give_their_pages_back_when_the_copy_fails():
+    from higgs_b200.engine import Sequence
+    eng = _engine_whose_copies_fail()
+    seq = Sequence(prompt=np.zeros(20, np.int32), pages=eng.pool.alloc(2).tolist(), length=20)
+    with pytest.raises(RuntimeError):
+        eng.fork(seq, 3)
+    assert eng.pool.num_free == 10 and [eng.pool.refcount(p) for p in seq.pages] == [1, 1]
+    with pytest.raises(RuntimeError):
+        eng._reorder([seq], [(0, 1, 0.0), (0, 2, 0.0), (0, 3, 0.0)])
+    assert eng.pool.num_free == 10 and [eng.pool.refcount(p) for p in seq.pages] == [1, 1]
+    eng.release(seq)
+    assert eng.pool.num_free == 12
