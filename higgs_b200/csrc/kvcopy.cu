@@ -93,6 +93,16 @@ int launch_copy(const higgs_kv_pool* pools, int n_pools, const int32_t* src, con
   return HIGGS_OK;
 }
 
+// No byte belongs to pages of two layers: a layer's pages before the next layer's, or the layers of a
+// page before the next page.
+bool layers_apart(const higgs_kv_pool& p) {
+  if (p.layers == 1) return true;
+  typedef __int128 wide;
+  const wide pages = p.num_pages == 1 ? 0 : (wide)(p.num_pages - 1) * p.page_stride;
+  return p.layer_stride >= p.page_bytes &&
+         (p.layer_stride >= pages + p.page_bytes || p.page_stride >= (wide)(p.layers - 1) * p.layer_stride + p.page_bytes);
+}
+
 // The pairs fit the pools and commute: ids in range, no destination twice, none among the sources.
 int check_pairs(const int32_t* src, const int32_t* dst, int n, int64_t pages) {
   for (int i = 0; i < n; ++i)
@@ -128,6 +138,7 @@ extern "C" int higgs_kv_copy_pages(higgs_ctx* ctx, const higgs_kv_pool* pools, i
                  "higgs_kv_copy_pages: bases, strides and page sizes must be multiples of 16 bytes");
     HG_CHECK_ARG(p.num_pages == 1 || p.page_stride >= p.page_bytes,
                  "higgs_kv_copy_pages: pages overlap");
+    HG_CHECK_ARG(layers_apart(p), "higgs_kv_copy_pages: layers overlap");
     HG_CHECK_ARG(p.page_bytes <= (int64_t)1 << 30, "higgs_kv_copy_pages: page larger than 1 GiB");
     pages = std::min(pages, p.num_pages);
   }

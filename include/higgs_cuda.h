@@ -407,8 +407,9 @@ int higgs_window_attention(higgs_ctx* ctx, const void* q, int B, int Lq, int Hq,
  * it, page dst[i] becomes page src[i], i < n.  A pool is one tensor of the cache -- K
  * or V, or a TurboQuant cache's codes and scales -- with page p of layer l at
  * base + l * layer_stride + p * page_stride, page_bytes long (bytes; base, strides and
- * page_bytes multiples of 16; num_pages bounds the ids); 1 to 8 pools that do not
- * overlap.
+ * page_bytes multiples of 16; num_pages bounds the ids); all pages of a layer lie before
+ * the next layer's, or all layers of a page before the next page's; 1 to 8 pools that do
+ * not overlap.
  *   src and dst are HOST lists (page ids come from the host's block pool), read before
  *   the call returns; a captured graph keeps the lists it was captured with.  A source
  *   may feed several destinations; a page that is a destination twice, or a source and

@@ -203,3 +203,20 @@ def test_forks_give_their_pages_back_when_the_copy_fails():
     assert eng.pool.num_free == 10 and [eng.pool.refcount(p) for p in seq.pages] == [1, 1]
     eng.release(seq)
     assert eng.pool.num_free == 12
+
+
+def test_kv_copy_refuses_overlapping_layers(lib):
+    """Layers apart, or interleaved within a page's stride; nothing that would race."""
+    def call(layers, pages, layer_stride, page_stride, page_bytes=64):
+        words = (ctypes.c_int64 * 6)(4096, layers, pages, layer_stride, page_stride, page_bytes)
+        return lib.higgs_kv_copy_pages(4096, words, 1, 4096, 4096, 0, None)
+    assert call(3, 10, 640, 64) == 0     # [layers, pages]
+    assert call(3, 10, 64, 192) == 0     # [pages, layers]
+    assert call(1, 10, 0, 64) == 0       # one layer: its stride is not used
+    assert call(3, 1, 64, 0) == 0        # one page: nor is the pages'
+    for bad in ((3, 10, 0, 64), (3, 10, 576, 64), (3, 10, 64, 176), (3, 10, 48, 192), (2, 10, -640, 64),
+                (2, 2 ** 62, 64, 64), (2, 10, 64, 2 ** 62)):
+        rc = call(*bad)
+        assert rc == (0 if bad == (2, 10, 64, 2 ** 62) else -1), bad
+        if rc:
+            assert "overlap" in _err(lib), bad
