@@ -174,6 +174,13 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         return lib
 
 
+def fits_int(*sizes) -> None:
+    """Refuses sizes that the C interface's 32-bit ints would cut."""
+    for n in sizes:
+        if not -0x80000000 <= n <= 0x7fffffff:
+            raise ValueError(f"{n} does not fit 32 bits")
+
+
 def call(name: str, *args) -> int:
     lib = _lib or load()
     rc = getattr(lib, name)(*args)

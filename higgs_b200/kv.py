@@ -53,6 +53,7 @@ class BlockPool:
     def fork(self, pages, length: int) -> tuple[np.ndarray, tuple[int, int] | None]:
         """(pages of a second owner of the sequence, the (source, destination) pair of pages to copy
         or None): whole pages are shared, a partly filled last one is replaced by a fresh one."""
+        ffi.fits_int(length)
         p = np.ascontiguousarray(pages, dtype=np.int32)
         out = np.empty(-(-max(length, 0) // PAGE), np.int32)
         pair = np.empty(2, np.int32)
@@ -63,7 +64,7 @@ class BlockPool:
     def compact(self, max_moves: int | None = None) -> tuple[np.ndarray, np.ndarray]:
         """Packs allocated pages into the lowest ids; the moves (sources, destinations), whose
         pages the caller copies and renames."""
-        m = self.num_pages if max_moves is None else max_moves
+        m = self.num_pages if max_moves is None else min(max_moves, self.num_pages)
         moves = np.empty((2, max(m, 1)), np.int32)
         n = ctypes.c_int(0)
         ffi.call("higgs_block_pool_compact", self.handle, m, _i32p(moves[0]), _i32p(moves[1]), ctypes.byref(n))

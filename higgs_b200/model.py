@@ -328,6 +328,7 @@ class Model:
         attn_sinks ones (bf16 pages only)."""
         self.args = args
         self.attn_window, self.attn_sinks = int(attn_window), int(attn_sinks)
+        ffi.fits_int(self.attn_window, self.attn_sinks)
         self.device = torch.device(device)
         self.weights = weights
         self.kv_mode = kv_mode

@@ -293,6 +293,7 @@ def fused_attention(qkv, Hq: int, Hkv: int, D: int, q_norm_w, k_norm_w, eps: flo
 
 
 def window_attention_workspace(B, Lq, Hq, Hkv, D, max_seq_len, window, sinks, device) -> torch.Tensor:
+    ffi.fits_int(max_seq_len, window, sinks)
     n = ffi.load().higgs_window_attention_workspace_size(B, Lq, Hq, Hkv, D, max_seq_len, window, sinks)
     return torch.zeros(max(n, 16384), dtype=torch.uint8, device=device)
 
@@ -324,6 +325,7 @@ def window_attention(q, k_cache, v_cache, block_table, seq_lens, max_seq_len: in
         raise ValueError("block_table must be [B, max_blocks] and seq_lens [B]")
     if not (q.is_contiguous() and block_table.is_contiguous() and seq_lens.is_contiguous()):
         raise ValueError("q, block_table and seq_lens must be contiguous")
+    ffi.fits_int(max_seq_len, window, sinks)
     ctx = _ctx(q)
     _same_device(q, k_cache, v_cache, block_table, seq_lens, workspace)
     if workspace is None:
@@ -459,6 +461,7 @@ def logprobs(logits, temperature: float, tokens, top_n: int = 0):
 
 
 def beam_select_workspace(B: int, beams: int, V: int, n_out: int, device) -> torch.Tensor:
+    ffi.fits_int(n_out)
     n = ffi.load().higgs_beam_select_workspace_size(B, beams, V, n_out)
     return torch.zeros(max(n, 4096), dtype=torch.uint8, device=device)
 
@@ -479,6 +482,7 @@ def beam_select(logits, scores, n_out: int, workspace=None):
         raise ValueError(f"logits must hold {B} x {W} rows, got {list(logits.shape)}")
     if not (logits.is_contiguous() and scores.is_contiguous()):
         raise ValueError("logits and scores must be contiguous")
+    ffi.fits_int(n_out)
     ctx = _ctx(logits)
     _same_device(logits, scores, workspace)
     n_out = int(n_out)

@@ -220,3 +220,35 @@ def test_kv_copy_refuses_overlapping_layers(lib):
         assert rc == (0 if bad == (2, 10, 64, 2 ** 62) else -1), bad
         if rc:
             assert "overlap" in _err(lib), bad
+
+
+def test_sizes_past_32_bits_are_refused_not_cut():
+    """A size that does not fit the C interface's ints must not arrive as its lower half."""
+    import torch
+
+    from higgs_b200 import ops
+    from higgs_b200.model import Model, tiny_args
+    big = 2 ** 32 + 5
+    q = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16)
+    kv = torch.zeros(4, 1, 16, 64, dtype=torch.bfloat16)
+    bt, sl = torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    for args in ((big, 16, 0), (64, big, 0), (64, 16, big), (64, -big, 0), (64, 16, -big)):
+        with pytest.raises(ValueError, match="32 bits"):
+            ops.window_attention(q, kv, kv, bt, sl, *args)
+        with pytest.raises(ValueError, match="32 bits"):
+            ops.window_attention_workspace(1, 1, 2, 1, 64, *args, "cpu")
+    with pytest.raises(ValueError, match="32 bits"):
+        ops.beam_select(torch.zeros(2, 8), torch.zeros(1, 2), big)
+    with pytest.raises(ValueError, match="32 bits"):
+        ops.beam_select_workspace(1, 2, 8, big, "cpu")
+    for kw in (dict(attn_window=big), dict(attn_window=8, attn_sinks=big)):
+        with pytest.raises(ValueError, match="32 bits"):
+            Model(tiny_args("qwen3", 1), {}, num_pages=4, **kw)
+    pool = BlockPool(4)
+    with pytest.raises(ValueError, match="32 bits"):
+        pool.fork(pool.alloc(1), big)
+    src, _ = pool.compact(big)  # more than there are pages: all
+    assert src.size == 0
+    pool.alloc(1)
+    pool.release([0])
+    assert [x.tolist() for x in pool.compact(big)] == [[1], [0]]
