@@ -11,7 +11,7 @@
 // the launch.  One warp moves one piece of a page, at most 4 KB: eight 16-byte loads per lane are
 // in flight before the first store, and the division of the piece's index is paid once per 4 KB.
 // B200: 500 pages of 36 layers (2.36 GB moved) 354 us = 6.67 TB/s; 77 pages of a 4-bit cache (94 MB)
-// 16.9 us = 5.5 TB/s, start and drain included; four pages 3 us, of which most is the launch.
+// 16.9 us = 5.5 TB/s, start and drain included; four pages of 28 layers 3.8 us, of which most is the launch.
 #include <algorithm>
 #include <new>
 #include <vector>
