@@ -194,9 +194,9 @@ union BeamShared {
   JoinShared join;
 };
 
-// A bound that n or more (and mostly few more) of the m values reach; the least of them, or 1, if
-// there are fewer than n.  Zeros do not count.  Each pass spreads the range that holds the n-th
-// value over 256 bins.
+// A bound that n or more (and mostly few more) of the m values reach, or 1, which bounds nothing, if
+// there are fewer than n: the least of them is no bound for what the values are the heads of.  Zeros
+// do not count.  Each pass spreads the range that holds the n-th value over 256 bins.
 __device__ __forceinline__ uint32_t block_bound(const uint32_t* v, int m, int n, BoundShared& sh) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -247,7 +247,7 @@ __device__ __forceinline__ uint32_t block_bound(const uint32_t* v, int m, int n,
     }
     if (threadIdx.x == 0) sh.total = c;
     __syncthreads();
-    if (sh.total < n) return lo;
+    if (sh.total < n) return 1;  // (in the first pass: later ones hold the n-th)
     lo += (uint32_t)sh.pick << shift;
     if (shift == 0 || sh.reach <= n + 8) return lo;
     hi = min(hi, lo + (1u << shift) - 1);
@@ -494,7 +494,8 @@ __device__ __forceinline__ void join_request(const BeamArgs& a, int b, JoinShare
   };
   // Few entries: a bound that hardly more than n of them reach, and a rank for each of those.  Many
   // (so many lists), or too many of one value: entries no better than the n-th of the lists' heads
-  // are left out, and the warps sort the rest.
+  // are left out -- none where fewer than n lists have one: dead beams and masked places have no
+  // list -- and the warps sort the rest.
   int count = kMaxCand + 1;
   if (direct) {
     BeamKey key[kMaxDirect / kBeamThreads];

@@ -223,3 +223,32 @@ def test_beam_select_two_streams():
                 got.append(ops().beam_select(xt, st, 16))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
+
+@pytest.mark.parametrize("B,W,V,n", [(4, 16, 151936, 32), (3, 16, 128256, 32), (2, 16, 151936, 32), (1, 32, 151936, 32),
+                                     (7, 32, 100001, 32), (5, 9, 151936, 18)])
+@pytest.mark.parametrize("live", [1, 2])
+def test_beam_select_few_beams_alive(B, W, V, n, live):
+    """The first step of wide beams, and beams that died: many lists, of which fewer than n hold anything."""
+    x, s = draw(B + W + V + live, B, W, V)
+    s[:, live:] = -np.inf
+    x[0, 1:live] = np.nan
+    check(x, s, n)
+
+
+@pytest.mark.parametrize("B,W,V,n,lo,hi", [(1, 8, 151936, 16, 1000, 1200), (2, 16, 151936, 32, 70000, 70033),
+                                           (1, 32, 128256, 32, 128255, 128256), (1, 16, 151935, 31, 4090, 4100)])
+@pytest.mark.parametrize("seed", [0, 1, 2])
+def test_beam_select_neighbouring_tokens_allowed(B, W, V, n, lo, hi, seed):
+    """A mask that leaves tokens in one or two places of the vocabulary: most lists are empty."""
+    x, s = draw(V + lo + seed, B, W, V)
+    x[:, :, :lo] = -np.inf
+    x[:, :, hi:] = -np.inf
+    check(x, s / 20, n)  # beams of similar scores: each list's best is near the others'
+
+
+def test_beam_select_many_equal_keys_behind_few_heads():
+    """More equal candidates than are ranked directly behind fewer than n lists' best ones."""
+    x = np.zeros((1, 20, 4096), np.float32)
+    x[:, :, 1000] = 5
+    check(x, np.full((1, 20), -1.0, np.float32), 32)
