@@ -336,13 +336,20 @@ extern "C" int higgs_block_pool_fork(higgs_block_pool* p, const int32_t* pages, 
   return HIGGS_OK;
 }
 
+// The free pages in the order that hands out the lowest first.
+static void list_free_pages(higgs_block_pool* p, std::vector<int32_t>& room) {
+  for (int32_t i = (int32_t)p->refcount.size() - 1; i >= 0; --i)
+    if (p->refcount[i] <= 0) room.push_back(i);
+  p->free_list.swap(room);
+}
+
 extern "C" int higgs_block_pool_compact(higgs_block_pool* p, int max_moves, int32_t* src, int32_t* dst,
                                         int* n_moves) try {
   if (!p || max_moves < 0 || (max_moves > 0 && (!src || !dst)) || !n_moves)
     return fail(HIGGS_ERR_INVALID_ARG, "higgs_block_pool_compact: bad argument");
   const int32_t pages = (int32_t)p->refcount.size();
-  std::vector<int32_t> free_list;
-  free_list.reserve((size_t)pages);
+  std::vector<int32_t> room;
+  room.reserve((size_t)pages);
   int n = 0;
   for (int32_t lo = 0, hi = pages - 1; n < max_moves; ++n) {
     while (lo < pages && p->refcount[lo] > 0) ++lo;
@@ -352,13 +359,31 @@ extern "C" int higgs_block_pool_compact(higgs_block_pool* p, int max_moves, int3
     dst[n] = lo;
     std::swap(p->refcount[lo], p->refcount[hi]);
   }
-  for (int32_t i = pages - 1; i >= 0; --i)  // the lowest free page is handed out first
-    if (p->refcount[i] <= 0) free_list.push_back(i);
-  p->free_list.swap(free_list);
+  list_free_pages(p, room);
   *n_moves = n;
   return HIGGS_OK;
 } catch (const std::bad_alloc&) {
   return fail(HIGGS_ERR_STATE, "higgs_block_pool_compact: out of host memory");
+}
+
+extern "C" int higgs_block_pool_move(higgs_block_pool* p, const int32_t* src, const int32_t* dst, int n) try {
+  if (!p || n < 0 || (n > 0 && (!src || !dst)))
+    return fail(HIGGS_ERR_INVALID_ARG, "higgs_block_pool_move: bad argument");
+  const int32_t pages = (int32_t)p->refcount.size();
+  std::vector<int32_t> room;
+  room.reserve((size_t)pages);
+  for (int i = 0; i < n; ++i) {
+    if (src[i] < 0 || src[i] >= pages || dst[i] < 0 || dst[i] >= pages || p->refcount[src[i]] <= 0 ||
+        p->refcount[dst[i]] > 0) {
+      while (i-- > 0) std::swap(p->refcount[src[i]], p->refcount[dst[i]]);
+      return fail(HIGGS_ERR_INVALID_ARG, "higgs_block_pool_move: needs an allocated source and a free destination");
+    }
+    std::swap(p->refcount[src[i]], p->refcount[dst[i]]);
+  }
+  list_free_pages(p, room);
+  return HIGGS_OK;
+} catch (const std::bad_alloc&) {
+  return fail(HIGGS_ERR_STATE, "higgs_block_pool_move: out of host memory");
 }
 
 // ---------------------------------------------------------------------------

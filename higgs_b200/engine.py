@@ -185,15 +185,19 @@ class Engine:
 
     def compact(self, seqs: list[Sequence], max_moves: int | None = None) -> int:
         """Packs the pool's allocated pages into its lowest ids; `seqs` must be all sequences that
-        own pages.  Returns the number of pages moved."""
+        own pages.  Returns the number of pages moved.  When the copy fails nothing is changed."""
         src, dst = self.pool.compact(max_moves)
         if not src.size:
             return 0
-        self._copy_pages(src, dst)
+        try:
+            self._copy_pages(src, dst)
+            self.prefix.remap(src, dst)
+        except Exception:
+            self.pool.move(dst, src)
+            raise
         to = dict(zip(src.tolist(), dst.tolist()))
         for s in seqs:
             s.pages = [to.get(p, p) for p in s.pages]
-        self.prefix.remap(src, dst)
         return int(src.size)
 
     # ---- prefill -------------------------------------------------------------------------

@@ -70,6 +70,15 @@ class BlockPool:
         ffi.call("higgs_block_pool_compact", self.handle, m, _i32p(moves[0]), _i32p(moves[1]), ctypes.byref(n))
         return moves[0, :n.value].copy(), moves[1, :n.value].copy()
 
+    def move(self, src, dst) -> None:
+        """Moves the counts of allocated pages src[i] to free pages dst[i]; move(dst, src) takes
+        back the moves that compact returned."""
+        s = np.ascontiguousarray(src, dtype=np.int32)
+        d = np.ascontiguousarray(dst, dtype=np.int32)
+        if s.size != d.size:
+            raise ValueError("move: lists of different lengths")
+        ffi.call("higgs_block_pool_move", self.handle, _i32p(s), _i32p(d), s.size)
+
 
 class PrefixCache:
     """PrefixCache (prompt_cache.rs:41-311) over whole KV pages."""

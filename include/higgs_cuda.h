@@ -749,6 +749,10 @@ int higgs_block_pool_fork(higgs_block_pool* pool, const int32_t* pages, int n_pa
  * the prefix cache, before any of the ids is used again. */
 int higgs_block_pool_compact(higgs_block_pool* pool, int max_moves, int32_t* src, int32_t* dst,
                              int* n_moves);
+/* Moves the counts of allocated pages src[i] to free pages dst[i], in this order; nothing is
+ * changed on an error.  With higgs_block_pool_compact's lists exchanged it takes the moves back,
+ * for a caller whose copies failed (compaction never writes to a source page). */
+int higgs_block_pool_move(higgs_block_pool* pool, const int32_t* src, const int32_t* dst, int n);
 
 /* PrefixCache (crates/higgs-engine/src/prompt_cache.rs:41-311) over pages:
  * a compressed radix trie of token ids whose entries hold page ids.  Only the

@@ -252,3 +252,40 @@ def test_sizes_past_32_bits_are_refused_not_cut():
     pool.alloc(1)
     pool.release([0])
     assert [x.tolist() for x in pool.compact(big)] == [[1], [0]]
+
+
+def test_compact_changes_nothing_when_the_copy_fails():
+    from higgs_b200.engine import Sequence
+    eng = _engine_whose_copies_fail()
+    eng.prefix = PrefixCache(eng.pool, 4)
+    hole = eng.pool.alloc(3)
+    seq = Sequence(prompt=np.zeros(40, np.int32), pages=eng.pool.alloc(3).tolist(), length=40)
+    toks = np.arange(32, dtype=np.int32)
+    eng.prefix.store(toks, np.array(seq.pages[:2], np.int32))
+    eng.pool.release(hole)
+    pages = list(seq.pages)
+    with pytest.raises(RuntimeError):
+        eng.compact([seq])
+    assert seq.pages == pages and [eng.pool.refcount(p) for p in pages] == [2, 2, 1]
+    assert eng.pool.num_free == 9 and eng.prefix.lookup(toks)[1].tolist() == pages[:2]
+    eng.pool.release(pages[:2])
+    eng.release(seq)  # the pages are still this sequence's
+    eng.prefix.clear()
+    assert eng.pool.num_free == 12
+
+
+def test_pool_move_takes_compaction_back_and_refuses():
+    pool = BlockPool(6)
+    pages = pool.alloc(6)
+    pool.retain(pages[5:])
+    pool.release(pages[:2])
+    src, dst = pool.compact()
+    pool.move(dst, src)
+    assert [pool.refcount(p) for p in range(6)] == [0, 0, 1, 1, 1, 2] and pool.num_free == 2
+    for s, d in (([2, 0], [1, 3]), ([2, 3], [0, 0]), ([2, 2], [0, 1]), ([0], [1]), ([6], [0]), ([-1], [0]), ([2], [6])):
+        with pytest.raises(HiggsError):
+            pool.move(s, d)
+        assert [pool.refcount(p) for p in range(6)] == [0, 0, 1, 1, 1, 2]
+    with pytest.raises(ValueError):
+        pool.move([2], [0, 1])
+    assert pool.alloc(2).tolist() == [0, 1]
