@@ -236,6 +236,14 @@ void remap(Node& n, const std::map<int32_t, int32_t>& to) {
   for (auto& kv : n.children) remap(*kv.second, to);
 }
 
+void count_uses(const Node& n, std::map<int32_t, int32_t>& uses) {
+  for (int32_t pg : n.pages) {
+    const auto it = uses.find(pg);
+    if (it != uses.end()) it->second++;
+  }
+  for (const auto& kv : n.children) count_uses(*kv.second, uses);
+}
+
 void release_all(higgs_prefix_cache* pc, Node& n) {
   if (n.cached) pool_release(pc->pool, n.pages);
   n.cached = false;
@@ -471,4 +479,16 @@ extern "C" int higgs_prefix_cache_remap(higgs_prefix_cache* pc, const int32_t* s
   return HIGGS_OK;
 } catch (const std::bad_alloc&) {
   return fail(HIGGS_ERR_STATE, "higgs_prefix_cache_remap: out of host memory");
+}
+
+extern "C" int higgs_prefix_cache_uses(const higgs_prefix_cache* pc, const int32_t* pages, int n, int32_t* uses) try {
+  if (!pc || n < 0 || (n > 0 && (!pages || !uses)))
+    return fail(HIGGS_ERR_INVALID_ARG, "higgs_prefix_cache_uses: bad argument");
+  std::map<int32_t, int32_t> count;
+  for (int i = 0; i < n; ++i) count[pages[i]] = 0;
+  count_uses(pc->root, count);
+  for (int i = 0; i < n; ++i) uses[i] = count[pages[i]];
+  return HIGGS_OK;
+} catch (const std::bad_alloc&) {
+  return fail(HIGGS_ERR_STATE, "higgs_prefix_cache_uses: out of host memory");
 }

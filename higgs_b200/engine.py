@@ -10,6 +10,7 @@ cache slot, length) are device vectors refreshed by one small host->device copy.
 """
 from __future__ import annotations
 
+import collections
 import dataclasses
 import math
 
@@ -185,11 +186,18 @@ class Engine:
 
     def compact(self, seqs: list[Sequence], max_moves: int | None = None) -> int:
         """Packs the pool's allocated pages into its lowest ids; `seqs` must be all sequences that
-        own pages.  Returns the number of pages moved.  When the copy fails nothing is changed."""
+        own pages (ValueError when a page to move has an owner that is neither among them nor in the
+        prefix cache).  Returns the number of pages moved; on an error nothing is changed."""
+        seqs = list({id(s): s for s in seqs}.values())
         src, dst = self.pool.compact(max_moves)
         if not src.size:
             return 0
         try:
+            owners = collections.Counter(p for s in seqs for p in s.pages)
+            for p, q, cached in zip(src.tolist(), dst.tolist(), self.prefix.uses(src).tolist()):
+                if owners[p] + cached != self.pool.refcount(q):
+                    raise ValueError(f"compact: page {p} has {self.pool.refcount(q)} owners, {owners[p]} among the "
+                                     f"{len(seqs)} sequences given and {cached} in the prefix cache")
             self._copy_pages(src, dst)
             self.prefix.remap(src, dst)
         except Exception:

@@ -99,6 +99,7 @@ SIGNATURES: dict[str, tuple] = {
     "higgs_block_pool_compact": (I, [P, I, P, P, ctypes.POINTER(I)]),
     "higgs_block_pool_move": (I, [P, P, P, I]),
     "higgs_prefix_cache_remap": (I, [P, P, P, I]),
+    "higgs_prefix_cache_uses": (I, [P, P, I, P]),
     "higgs_prefix_cache_create": (I, [P, I, ctypes.POINTER(P)]),
     "higgs_prefix_cache_destroy": (I, [P]),
     "higgs_prefix_cache_len": (I, [P]),

@@ -122,3 +122,10 @@ class PrefixCache:
         if s.size != d.size:
             raise ValueError("remap: lists of different lengths")
         ffi.call("higgs_prefix_cache_remap", self.handle, _i32p(s), _i32p(d), s.size)
+
+    def uses(self, pages) -> np.ndarray:
+        """How many references to each of the pages the entries hold."""
+        p = np.ascontiguousarray(pages, dtype=np.int32)
+        out = np.empty(p.size, np.int32)
+        ffi.call("higgs_prefix_cache_uses", self.handle, _i32p(p), p.size, _i32p(out))
+        return out

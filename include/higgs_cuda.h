@@ -776,6 +776,8 @@ int higgs_prefix_cache_store(higgs_prefix_cache* pc, const int32_t* tokens, int 
 /* Renames pages src[i] -> dst[i] in every entry, after higgs_block_pool_compact (which
  * moved their counts). */
 int higgs_prefix_cache_remap(higgs_prefix_cache* pc, const int32_t* src, const int32_t* dst, int n);
+/* uses[i]: how many references to page pages[i] the entries hold. */
+int higgs_prefix_cache_uses(const higgs_prefix_cache* pc, const int32_t* pages, int n, int32_t* uses);
 
 /* ---- (f)2: MLX-format safetensors model directories --------------------- */
 

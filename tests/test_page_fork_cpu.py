@@ -289,3 +289,31 @@ def test_pool_move_takes_compaction_back_and_refuses():
     with pytest.raises(ValueError):
         pool.move([2], [0, 1])
     assert pool.alloc(2).tolist() == [0, 1]
+
+
+def test_compact_refuses_when_a_sequence_is_missing():
+    """A sequence that is not named would keep the old ids of its moved pages."""
+    from higgs_b200.engine import Sequence
+    eng = _engine_whose_copies_fail()
+    eng._copy_pages = lambda src, dst: None
+    eng.prefix = PrefixCache(eng.pool, 4)
+    hole = eng.pool.alloc(2)
+    a, b = (Sequence(prompt=np.zeros(40, np.int32), pages=eng.pool.alloc(3).tolist(), length=40) for _ in range(2))
+    toks = np.arange(32, dtype=np.int32)
+    eng.prefix.store(toks, np.array(a.pages[:2], np.int32))
+    eng.prefix.store(np.concatenate([toks, toks]), np.array(a.pages[:2] + b.pages[:2], np.int32))
+    assert eng.prefix.uses(a.pages + b.pages + [99]).tolist() == [2, 2, 0, 1, 1, 0, 0]
+    shared = Sequence(prompt=a.prompt, pages=list(a.pages), length=40)
+    eng.pool.retain(a.pages)
+    eng.pool.release(hole)
+    before = [list(a.pages), list(b.pages), [eng.pool.refcount(p) for p in range(12)]]
+    for seqs in ([], [a], [a, b][:1], [a, shared]):
+        with pytest.raises(ValueError, match="owners"):
+            eng.compact(seqs)
+        assert before == [a.pages, b.pages, [eng.pool.refcount(p) for p in range(12)]]
+    assert eng.compact([a, b, shared, a]) == 2  # a sequence named twice is one
+    assert sorted(a.pages + b.pages) == list(range(6)) and shared.pages == a.pages
+    for s in (a, b, shared):
+        eng.release(s)
+    eng.prefix.clear()
+    assert eng.pool.num_free == 12
