@@ -439,13 +439,17 @@ class Engine:
                     logits = g.logits
                 if W not in ws:
                     ws[W] = ops.beam_select_workspace(1, W, V, n, dev)
-                best, par, tok = ops.beam_select(logits, torch.tensor([total], dtype=torch.float32).to(dev), n,
-                                                 workspace=ws[W])
+                # scores go to the device as distances from the best one: the sums stay in 64 bits, and a
+                # step's rounding to f32 is that of a distance
+                top = max(total)
+                behind = torch.tensor([[t - top for t in total]], dtype=torch.float32).to(dev)
+                best, par, tok = ops.beam_select(logits, behind, n, workspace=ws[W])
                 best, par, tok = (t.cpu().numpy()[0] for t in (best, par, tok))
                 chosen = []  # (parent, token, log-probability) that go on
                 for s, p, t in zip(best.tolist(), par.tolist(), tok.tolist()):
                     if p < 0 or len(chosen) == beams:
                         break
+                    s += top
                     if eos_token_id is not None and t == eos_token_id:
                         done.append((s / (step + 1) ** length_penalty, seqs[p].generated + [t]))
                     else:
