@@ -567,6 +567,9 @@ class SpecDecoder:
         self.fa_verify = m.forward_args(self.vtok, self.v_pos, self.v_slots, self.block_table,
                                         self.v_lens, msl, last_only=False,
                                         logits=self.target_logits.view(B * k1, V))
+        # until a step is staged nothing goes into the cache (slot 0 is some sequence's)
+        self.d_slots.fill_(-1)
+        self.v_slots.fill_(-1)
         self.graph = None
         if use_graph:
             s = torch.cuda.Stream(dev)

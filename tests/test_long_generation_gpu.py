@@ -208,3 +208,20 @@ def test_windowed_model_refuses_tq4(weights):
     from higgs_b200.ffi import HiggsError
     with pytest.raises(HiggsError, match="TurboQuant"):
         engine(weights, kv_mode="tq4", attn_window=16)
+
+
+@pytest.mark.parametrize("kv_mode,kw", [("bf16", {}), ("bf16", {"attn_window": 24}), ("tq4", {})])
+def test_speculative_decoder_made_late_leaves_the_cache(weights, kv_mode, kw):
+    """Making a SpecDecoder (its warm-up and capture) writes nothing into pages that sequences own."""
+    from higgs_b200.engine import SpecDecoder
+    eng = engine(weights, kv_mode=kv_mode, **kw)
+    seq = eng.prefill(prompt(40), use_prefix=False)
+    torch.cuda.synchronize()
+    before = [p.clone() for p in eng.model.kv_pools]
+    dec = SpecDecoder(eng, 2, k=3, draft_layers=1, temperature=0.0)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(before, eng.model.kv_pools))
+    dec.stage([seq, eng.fork(seq)[0]], np.zeros(2 * 3 * 2 + 2, np.float32), first=True)
+    dec.graph.replay()
+    torch.cuda.synchronize()
+    assert not all(torch.equal(a, b) for a, b in zip(before, eng.model.kv_pools))
