@@ -643,6 +643,7 @@ class SpecDecoder:
         v_slots = np.zeros((B, k1), np.int64)
         for b, s in enumerate(seqs):
             before = len(s.pages)
+            eng._trim(s)
             eng._ensure_pages(s, s.length + k1)
             if len(s.pages) != before or first:
                 self.bt_host[b, :len(s.pages)] = s.pages

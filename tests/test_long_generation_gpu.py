@@ -225,3 +225,28 @@ def test_speculative_decoder_made_late_leaves_the_cache(weights, kv_mode, kw):
     dec.graph.replay()
     torch.cuda.synchronize()
     assert not all(torch.equal(a, b) for a, b in zip(before, eng.model.kv_pools))
+
+
+def test_window_speculative_steps_give_up_pages(weights):
+    """Speculative steps of a windowed model: the same tokens whether the pages behind the window go
+    back to the pool (where another sequence takes and fills them) or stay."""
+    from higgs_b200.engine import SpecDecoder
+    runs = []
+    for trim in (True, False):
+        eng = engine(weights, attn_window=24, attn_sinks=4)
+        if not trim:
+            eng._trim = lambda s: None
+        seqs = [eng.prefill(prompt(n, seed=n), use_prefix=False) for n in (90, 40)]
+        dec = SpecDecoder(eng, 2, k=3, draft_layers=1, temperature=0.0)
+        rng = np.random.default_rng(0)
+        dec.steps(seqs, 8, rng)
+        other = eng.prefill(prompt(100, seed=9), use_prefix=False)  # fills the pages that were given up
+        acc = dec.steps(seqs, 8, rng)
+        live = [sum(p >= 0 for p in s.pages) for s in seqs]
+        if trim:  # sinks, window and the tokens ahead
+            assert max(live) <= 1 + 4 and all(s.pages[2] == -1 for s in seqs[:1])
+        runs.append(([list(s.generated) for s in seqs], acc))
+        for s in seqs + [other]:
+            eng.release(s)
+        assert eng.pool.num_free == 128
+    assert runs[0][0] == runs[1][0] and np.array_equal(runs[0][1], runs[1][1])

@@ -317,3 +317,46 @@ def test_compact_refuses_when_a_sequence_is_missing():
         eng.release(s)
     eng.prefix.clear()
     assert eng.pool.num_free == 12
+
+
+def test_speculative_steps_give_up_pages_behind_the_window():
+    """A windowed model's pages behind the window go back to the pool at speculative steps too, and the
+    slots and lengths of the step stay those of the untrimmed sequence."""
+    import types
+
+    import torch
+
+    from higgs_b200.engine import Engine, Sequence, SpecDecoder
+    B, k, pages = 2, 3, 40
+
+    def staged(window, lengths):
+        eng = Engine.__new__(Engine)
+        eng.pool = BlockPool(pages)
+        eng.model = types.SimpleNamespace(attn_window=window, attn_sinks=4)
+        dec = SpecDecoder.__new__(SpecDecoder)
+        dec.engine, dec.B, dec.k = eng, B, k
+        n = 4 * k * B + 3 * B * (k + 1) + B + 2 * k * B + B
+        dec.step_host, dec.step_dev = (torch.zeros(n, dtype=torch.int32) for _ in range(2))
+        dec.block_table = torch.zeros(B, 20, dtype=torch.int32)
+        dec.bt_host = np.zeros((B, 20), np.int32)
+        dec.tok = torch.zeros(k + 1, B, dtype=torch.int32)
+        seqs = [Sequence(prompt=np.zeros(1, np.int32), length=n, last_token=1) for n in lengths]
+        for s in seqs:
+            eng._ensure_pages(s, s.length)
+        steps = []
+        for it in range(12):
+            dec.stage(seqs, np.zeros(2 * k * B + B, np.float32), first=it == 0)
+            steps.append([[s.length, [s.pages[(s.length + i) // 16] >= 0 for i in range(k + 1)]] for s in seqs])
+            for s in seqs:
+                s.length += 3
+        return eng, seqs, steps
+
+    eng, seqs, steps = staged(24, [90, 7])
+    _, _, want = staged(0, [90, 7])
+    assert steps == want and all(all(x[1]) for st in steps for x in st)
+    # 123 + 4 tokens: page 0 (sinks) and those from key 123 - 23 on, 40 + 4: page 0 and from key 17 on
+    assert [[i for i, p in enumerate(s.pages) if p >= 0] for s in seqs] == [[0, 6, 7], [0, 1, 2]]
+    assert eng.pool.num_free == pages - 6
+    for s in seqs:
+        eng.release(s)
+    assert eng.pool.num_free == pages
