@@ -252,3 +252,16 @@ def test_beam_select_many_equal_keys_behind_few_heads():
     x = np.zeros((1, 20, 4096), np.float32)
     x[:, :, 1000] = 5
     check(x, np.full((1, 20), -1.0, np.float32), 32)
+
+
+@pytest.mark.parametrize("V", [3 * 4096 + 100, 3 * 4096 + 101])
+@pytest.mark.parametrize("thread", [0, 77, 255])
+def test_beam_select_all_of_one_thread(V, thread):
+    """Every candidate in the logits that one thread of the scan loads: with 16-byte loads four
+    neighbours of every 1024, else one of every 256."""
+    x, s = draw(V + thread, 2, 2, V, sd=1.0)
+    at = np.arange(V)
+    mine = (at % 1024) // 4 == thread if V % 4 == 0 else at % 256 == thread
+    x[:, :, mine] += 20
+    got = check(x, s, 32)
+    assert mine[got[2]].all()

@@ -250,3 +250,30 @@ def test_window_speculative_steps_give_up_pages(weights):
             eng.release(s)
         assert eng.pool.num_free == 128
     assert runs[0][0] == runs[1][0] and np.array_equal(runs[0][1], runs[1][1])
+
+
+@pytest.mark.parametrize("kv_mode,length", [("bf16", 37), ("bf16", 48), ("tq4", 37)])
+def test_forks_that_go_apart_are_sequences_of_their_own(weights, kv_mode, length):
+    """Three forks fed different tokens give, bit for bit, the logits of three sequences that never
+    shared a page (the same batch, so the same kernels)."""
+    force = np.stack([prompt(40, seed=s) for s in (1, 2, 3)])
+    runs = []
+    for forked in (True, False):
+        eng = engine(weights, kv_mode=kv_mode)
+        if forked:
+            first = eng.prefill(prompt(length), use_prefix=False)
+            seqs = [first] + eng.fork(first, 2)
+        else:
+            seqs = [eng.prefill(prompt(length), use_prefix=False) for _ in range(3)]
+        eng.step_logits.clear()
+        eng.decode_steps(seqs, 20, force=force[:, :20])
+        if forked:  # the first one's place is taken by a fork of it, made in the middle
+            seqs = eng.fork(seqs[0]) + seqs[1:]
+            eng.release(first)
+        eng.decode_steps(seqs, 20, force=force[:, 20:])
+        runs.append(np.stack(eng.step_logits))
+        for s in seqs:
+            eng.release(s)
+        assert eng.pool.num_free == 128
+    assert np.array_equal(runs[0], runs[1])
+    assert not np.array_equal(runs[0][-1, 0], runs[0][-1, 1])
