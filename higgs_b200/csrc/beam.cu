@@ -15,9 +15,11 @@
 // collects 32 sorts them (a bitonic network) and keeps the best, so no order of the logits needs
 // more room; at the end the CTA's few candidates are ranked by counting those above each.
 //
-// The CTA that completes a request's last round joins its lists, on keys in 64 bits: which of two
-// near candidates wins is decided by the difference of two log sums.  A histogram over the leading
-// bits bounds the n-th best, and what reaches the bound is ranked as above.
+// The CTA that completes a request's last round joins its lists.  A row's exponentials and their sums
+// are in f32 (a few ulps each; the log sum is held to 2^-20 by the tests), the logarithm, the key and
+// its order in 64 bits: candidates of two beams closer than the log sums' error may change places,
+// candidates of one beam or of equal rows never.  A histogram over the leading bits bounds the n-th
+// best, and what reaches the bound is ranked as above.
 //
 // Keys are unique (value, then index), and the sums of a round depend on its logits alone and are
 // added in the order of the rounds: equal rows give equal keys, and results do not depend on
@@ -27,7 +29,8 @@
 // logits, 32 best (311 MB) 73 us = 4.3 TB/s: nine CTAs in ten end their scans 48 to 62 us after the
 // start (equal shares, unequal speeds), and the last one's list and join take 10 more; 8 x 8 beams,
 // 16 best (39 MB) 19.7 us; one request 8.6 us, a chain of launch, one round, list, counter, log
-// sums and join.
+// sums and join.  Where fewer than n lists of more than 2048 entries hold anything (the first step of
+// wide beams), the join walks all entries: 32 us for 4 x 16 beams, 32 best; 64 us for 1 x 32.
 #include <algorithm>
 
 #include "common.cuh"

@@ -18,12 +18,23 @@
 // and 128 of O.  S_u+1 waits there while the softmax of S_u runs, S_u+2 is issued when P_u V_u is done.
 // Both halves share every K and V tile.
 //
-// Bound: the softmax warps, about 1950 cycles per half block of 64 keys and warpgroup, of which some
-// 1050 are its exponentials (both halves share the SM's 16 a cycle).  B200, 32 / 8 heads, D = 128:
-// 8192 tokens, window 4096, 370 us = 1117 TFLOP/s, 0.65 of a large product's burst rate; 2048 tokens,
-// window 1024, 54 us, 256 tiles on 148 SMs.  Measured slower for the 8192 tokens, against the kernel
-// of the time: 128-row tiles 790 (586); whole 128-key blocks with the product begun early 409 (378);
-// the halves half a step apart 380 (378); one warp issuing scores and products 374 (367).
+// P is rounded to bf16: one product per half block and not the two of the decode kernel's hi + lo
+// halves, and no columns of tensor memory beyond S's; the weights' errors (2^-9 each, of either sign)
+// average out over the keys of a prompt: 0.0023 of the output's norm from the 64-bit result, where the
+// rounding of the output alone makes 0.0017 (2048 tokens; 0.0022 and 0.0016 for 8192).
+//
+// Bound: the serial chain of a softmax warp -- scores from tensor memory, mask, maximum, vote,
+// exponentials, pack, store, arrive -- about 1950 cycles per half block of 64 keys and warpgroup; its
+// exponentials alone are some 1050 of them (both halves share the SM's 16 a cycle).  B200, 32 / 8
+// heads, D = 128, 8192 tokens, window 4096: 0.72 million cycles, that is 369 us at 1965 MHz (1118
+// TFLOP/s, 0.65 of a large product's burst rate) and 428 us in a loop of seconds, where the power cap
+// holds the clock at 1670 MHz (964 TFLOP/s, 0.67 of the product's sustained rate).  2048 tokens,
+// window 1024: 54 us at 1965 MHz, 256 tiles on 148 SMs.  Measured slower for the 8192 tokens, against
+// the kernel of the time: 128-row tiles 790 (586); whole 128-key blocks with the product begun early
+// 409 (378); the halves half a step apart 380 (378); one warp issuing scores and products 374 (367).
+// Few tiles: a tile's keys are not shared out, so a chunk of 17 to 512 tokens (8 to 64 tiles) behind
+// 1024 / 4096 / 8192 visible keys takes 26-29 / 70-74 / 129-134 us, all of it one CTA's walk; tiles of
+// at most 128 rows run their empty second half too.
 // Every mbarrier wait is bounded (about 2 s; the first timeout makes the CTA's other waits give up
 // and sets the flag that higgs_tc_error reports; copies and products in flight are then still waited for).
 #include <algorithm>

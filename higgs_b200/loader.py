@@ -31,7 +31,9 @@ def load_model_args(model_dir: str) -> ModelArgs:
     """ModelArgs from config.json.  Defaults follow the reference's serde defaults (rope_theta
     10000, tie_word_embeddings false); head_dim is the config's when given, else
     hidden_size / num_attention_heads (transformer.rs:117-126).  Only MLX affine 4-bit,
-    group-64 quantized checkpoints are accepted (the quantization block of config.json)."""
+    group-64 quantized checkpoints are accepted (the quantization block of config.json).
+    A sliding_window there is not read (the reference's ModelArgs has no such field and attends to
+    all keys): pass it to Model as attn_window."""
     with open(os.path.join(model_dir, "config.json")) as f:
         c = json.load(f)
     q = c.get("quantization")

@@ -325,7 +325,7 @@ class Model:
         """With `tp`, `weights` are this rank's shard (shard_weights) and the model is one
         rank of a tensor-parallel group: greedy tokens are identical on every rank.  With
         `attn_window`, every layer attends to the last attn_window keys and the first
-        attn_sinks ones (bf16 pages only)."""
+        attn_sinks ones (bf16 pages only); without it to all keys, attn_sinks or not."""
         self.args = args
         self.attn_window, self.attn_sinks = int(attn_window), int(attn_sinks)
         ffi.fits_int(self.attn_window, self.attn_sinks)

@@ -387,8 +387,9 @@ int higgs_paged_attention_noalloc(higgs_ctx* ctx, const void* q, int B, int Lq, 
  *   query of the call sees must be finite.
  *   D = 64 or 128; Hq / Hkv any whole number.  Base pointers and (positive) strides
  *   must be multiples of 16 bytes.  More than 64 query rows per kv head, Hq / Hkv * Lq,
- *   run on the tensor cores (option "attn_prefill_tc"), whose waits are bounded
- *   (higgs_tc_error).  workspace: at least
+ *   run on the tcgen05 tensor cores (option "attn_prefill_tc"), whose waits are bounded
+ *   (higgs_tc_error); the softmax weights are rounded to bf16 there, as in
+ *   higgs_paged_attention's prompts, and carry 16 bits with fewer rows.  workspace: at least
  *   higgs_window_attention_workspace_size() bytes (0 for a shape that is refused),
  *   zero-filled before its first use; each call leaves its counters (the first 16384
  *   bytes) zero, so calls of any shapes that follow one another on a stream can share
@@ -526,8 +527,11 @@ int higgs_apply_token_mask(higgs_ctx* ctx, float* logits, int B, int V, const ui
  * best continuations by
  *   key(w, v) = scores[b, w] + logits[b, w, v] - log sum_u exp(logits[b, w, u]),
  * best first, ties to the lower w * V + v.  logits f32 [B * beams, V]; scores f32
- * [B, beams], the beams' log-probabilities so far; out_scores f32 (keys computed in 64
- * bits and rounded once), out_beams int32 (w) and out_tokens int32 (v), [B, n_out].
+ * [B, beams], the beams' log-probabilities so far; out_scores f32, out_beams int32 (w)
+ * and out_tokens int32 (v), [B, n_out].  The log sum is of f32 exponentials added in f32,
+ * good to about 2^-20; keys are formed and ordered in 64 bits and rounded once.  So near
+ * candidates of different beams are in the order of those log sums, equal rows' and one
+ * row's candidates in the exact one.
  *   A NaN logit counts as -inf: no mass, never chosen.  A beam whose score is not
  *   finite, or whose row has no finite maximum, gives no candidates and its row is not
  *   read (so the first step of a search sets all scores but one to -inf).  Where fewer
